@@ -23,6 +23,8 @@ reference computes on the CPU) are validated like any other call and then
 raise :class:`NoHostPathError`, a ``RuntimeError``.
 """
 
+from typing import NamedTuple
+
 import numpy as np
 
 from . import _fusedtok
@@ -34,7 +36,8 @@ except ImportError:  # pragma: no cover - torch is optional for the staged route
 
 __version__ = "0.2.0"
 __all__ = ["attention_decode", "attention_decode_paged", "attention_prefill", "kv_append", "kv_append_paged",
-           "rope", "rope_kv_append", "rope_kv_append_paged", "cuda_available", "NoHostPathError"]
+           "rope", "rope_kv_append", "rope_kv_append_paged", "attention_decode_paged_q8", "kv_append_paged_q8",
+           "block_table_extend", "block_table_trim", "BlockTableStep", "cuda_available", "NoHostPathError"]
 
 
 class NoHostPathError(RuntimeError):
@@ -542,3 +545,192 @@ def rope_kv_append_paged(q, k_pool, v_pool, block_table, k_new, v_new, lens, *, 
                 k_new.data_ptr(), v_new.data_ptr(), table.data_ptr(), pos.data_ptr(), k_pool.data_ptr(),
                 v_pool.data_ptr(), b, hq, hkv, d, page, table.shape[1], theta, pos_offset)
     return q_out
+
+
+# ---------------------------------------------------------------------------
+# paged cache held in 8 bits
+# ---------------------------------------------------------------------------
+
+# code type of the pools -> store code of the C ABI
+_CODES = {} if torch is None else {torch.int8: 0, torch.float8_e4m3fn: 1}
+_q8_workspace = {}       # (device, shape) -> bytes of workspace the launcher asks for
+
+
+def _q8_operands(lead, k_pool, v_pool, kv_scales, **rest):
+    """Checks common to the operators on an 8-bit paged cache: activations `rest` of one storage type, pools of one
+    code type, float32 scales, everything contiguous on one device. Returns (call, store, Nb, Hkv, P, D)."""
+    if not _on_gpu(lead):
+        raise TypeError("the operators on an 8-bit cache work on CUDA tensors only")
+    call = _DeviceCall(**rest)
+    for name, t, allowed in (("k_pool", k_pool, _CODES), ("v_pool", v_pool, _CODES),
+                             ("kv_scales", kv_scales, (torch.float32,))):
+        if not _on_gpu(t):
+            raise TypeError(f"{name}: a CUDA tensor is required")
+        if t.dtype not in allowed:
+            names = ", ".join(str(d).replace("torch.", "") for d in allowed)
+            raise TypeError(f"{name}: dtype {t.dtype} is not supported here (one of {names})")
+        if t.device != call.device:
+            raise TypeError(f"{name}: on {t.device} while the other operands are on {call.device}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name}: a contiguous tensor is required")
+    if v_pool.dtype is not k_pool.dtype:
+        raise TypeError(f"v_pool: dtype {v_pool.dtype} differs from k_pool's {k_pool.dtype}")
+    if k_pool.ndim != 4:
+        raise ValueError(f"k_pool: {k_pool.ndim}-D tensor where [Nb, Hkv, P, D] is expected")
+    if v_pool.shape != k_pool.shape:
+        raise ValueError(f"v_pool: shape {tuple(v_pool.shape)} differs from k_pool's {tuple(k_pool.shape)}")
+    blocks, hkv, page, dim = k_pool.shape
+    if kv_scales.shape != (blocks, hkv, 2):
+        raise ValueError(f"kv_scales: shape {tuple(kv_scales.shape)} where {(blocks, hkv, 2)} follows from the pools")
+    if page < 1:
+        raise ValueError("k_pool: blocks of at least one row are required")
+    return call, _CODES[k_pool.dtype], blocks, hkv, page, dim
+
+
+def attention_decode_paged_q8(q, k_pool, v_pool, kv_scales, block_table, lens=None):
+    """``attention_decode_paged`` over a cache held in 8 bits with one scale per block and kv head:
+
+    ``out[b, h] = softmax_t(ks[t] * (q[b, h] . k8[t]) / sqrt(D)) . (vs[t] * v8[t])``, t over the sequence's rows
+
+    q ``[B, Hq, D]`` float32, bfloat16 or float16 (the result has its type, accumulation is float32); pools
+    ``[Nb, Hkv, P, D]`` of ``torch.int8`` or ``torch.float8_e4m3fn`` codes; kv_scales ``[Nb, Hkv, 2]`` float32: K's
+    scale, then V's (``kv_append_paged_q8`` fills both); block_table ``[B, S]`` and lens ``[B]`` as in
+    ``attention_decode_paged``. Any GQA group. CUDA tensors only; host table and lens values are checked, CUDA
+    tensors trusted. The scratch of a call comes from torch's allocator, so calls on different streams do not share
+    any. No counterpart in the reference."""
+    call, store, blocks, hkv, page, dim = _q8_operands(q, k_pool, v_pool, kv_scales, q=q)
+    b, hq, d = call.dims("q", "B Hq D")
+    if d != dim:
+        raise ValueError(f"k_pool: head dim {dim} differs from q's {d}")
+    _gqa_heads(hq, hkv)
+    table = call.index("block_table", block_table, (b, None), blocks, False)
+    width = table.shape[1]
+    lens_dev = None if lens is None else call.index("lens", lens, (b,), width * page, True)
+    out = call.new((b, hq, d))
+    if b:
+        key = (call.device, call.code, b, hq, hkv, page, width, d)
+        need = _q8_workspace.get(key)
+        if need is None:
+            with torch.cuda.device(call.device):
+                need = _q8_workspace[key] = _fusedtok.attention_decode_paged_q8_workspace(*key[1:])
+        scratch = torch.empty(need, dtype=torch.uint8, device=call.device)
+        call.launch(_fusedtok.attention_decode_paged_q8_launch, call.code, store, q.data_ptr(), k_pool.data_ptr(),
+                    v_pool.data_ptr(), kv_scales.data_ptr(), table.data_ptr(),
+                    None if lens_dev is None else lens_dev.data_ptr(), out.data_ptr(), scratch.data_ptr(), need, b, hq,
+                    hkv, page, width, blocks, d)
+    return out
+
+
+def kv_append_paged_q8(k_pool, v_pool, kv_scales, k_new, v_new, slots):
+    """Round new tokens into an 8-bit paged cache, in place: ``k_new[i]`` / ``v_new[i]`` (``[N, Hkv, D]`` float32,
+    bfloat16 or float16) become row ``slots[i] % P`` of block ``slots[i] // P``; a negative slot passes its token over.
+    Pools and scales as in ``attention_decode_paged_q8``. Returns None.
+
+    All tokens of one call that go to one block have to have consecutive slots, in order (the slot map of
+    ``block_table_extend`` has). Per kv head, and for K and V each, with ``o`` the first of those rows and M = 127
+    (int8) or 448 (e4m3): ``old = scale if o > 0 else 0; new = max(old, max|x| / M)``; rows before ``o`` get the codes
+    ``round(code * old / new)``, the new ones ``round(x / new)`` (to the nearest code, ties to even); rows behind stay.
+    A value that is not finite makes the block's scale NaN. CUDA tensors only; host slots are checked (``< Nb * P``,
+    and the rule above), a CUDA tensor is trusted (slots outside the pool are passed over). No counterpart in the
+    reference."""
+    call, store, blocks, hkv, page, dim = _q8_operands(k_pool, k_pool, v_pool, kv_scales, k_new=k_new, v_new=v_new)
+    n, nh, nd = call.dims("k_new", "N Hkv D")
+    call.same_shape("v_new", "k_new")
+    if (nh, nd) != (hkv, dim):
+        raise ValueError(f"k_new: [Hkv, D] = {(nh, nd)} differs from the cache's {(hkv, dim)}")
+    if blocks * page > 0x7fffffff:
+        raise ValueError(f"k_pool: {blocks} blocks of {page} rows are more rows than a slot can name")
+    if not _on_gpu(slots):
+        slots = _host_slots(slots, n, blocks, page)
+    where = call.index("slots", slots, (n,), blocks * page, False) if _on_gpu(slots) else torch.from_numpy(slots).to(call.device)
+    if n:
+        call.launch(_fusedtok.kv_append_paged_q8_launch, call.code, store, k_new.data_ptr(), v_new.data_ptr(),
+                    where.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), kv_scales.data_ptr(), n, hkv, dim, page,
+                    blocks)
+    return None
+
+
+def _host_slots(slots, n, blocks, page):
+    """Slots given on the host, checked, as an int32 array."""
+    raw = slots.detach().numpy() if torch.is_tensor(slots) else np.asarray(slots)
+    if raw.size and raw.dtype.kind not in "iu":
+        raise TypeError(f"slots: integer values expected, found {raw.dtype}")
+    _index_shape("slots", raw.shape, (n,))
+    raw = raw.astype(np.int64)
+    if raw.size and int(raw.max()) >= blocks * page:
+        raise ValueError(f"slots: values must lie below {blocks * page} (found {int(raw.max())})")
+    raw = np.where(raw < 0, -1, raw)
+    # first token of each run; no block may have two
+    inside = (raw[1:] == raw[:-1] + 1) & (raw[1:] % page != 0) & (raw[:-1] >= 0)
+    begins = raw[np.concatenate([raw[:1] >= 0, ~inside & (raw[1:] >= 0)])] // page
+    if len(np.unique(begins)) != len(begins):
+        raise ValueError("slots: the tokens that go to one block must have consecutive slots, in order")
+    return raw.astype(np.int32)
+
+
+# ---------------------------------------------------------------------------
+# block tables
+# ---------------------------------------------------------------------------
+
+class BlockTableStep(NamedTuple):
+    """What ``block_table_extend`` returns, int32 CUDA tensors: ``slots [max_tokens]`` (block * P + offset of every new
+    token, -1 where there is none), ``starts [B + 1]`` (first token of each sequence among them), ``lens [B]`` (the
+    new lengths) and ``free_count [1]`` (blocks left on the free stack)."""
+    slots: object
+    starts: object
+    lens: object
+    free_count: object
+
+
+def _table_operands(block_table, page, **rest):
+    """Operands of the block table operators: contiguous int32 CUDA tensors of one device (they hold the state of the
+    cache, so nothing is converted). Returns (call, B, S)."""
+    if not _on_gpu(block_table):
+        raise TypeError("the block table operators work on CUDA tensors only")
+    call = _DeviceCall(dtypes=(torch.int32,), block_table=block_table, **rest)
+    b, width = call.dims("block_table", "B S")
+    for name in ("lens", "new_lens", "keep_lens"):
+        if name in rest:
+            _index_shape(name, rest[name].shape, (b,))
+    _index_shape("free_blocks", rest["free_blocks"].shape, (None,))
+    _index_shape("free_count", rest["free_count"].shape, (1,))
+    if int(page) != page or page < 1:
+        raise ValueError(f"page {page}: blocks of at least one row are required")
+    return call, b, width
+
+
+def block_table_extend(block_table, lens, new_lens, free_blocks, free_count, page, max_tokens):
+    """Blocks and slots for the next tokens of a paged cache, from the request lengths on the GPU.
+
+    block_table ``[B, S]`` is extended in place so that sequence b, which holds ``lens[b]`` tokens, can take
+    ``new_lens[b]`` more; the blocks come off the top of the free stack ``free_blocks[:free_count]`` in batch order
+    (the k-th one asked for is ``free_blocks[free_count - 1 - k]``). Returns a :class:`BlockTableStep`. The tokens are
+    numbered in batch order; ``max_tokens`` fixes the length of the slot map, so that a call can be captured.
+
+    A sequence that would outgrow its table row or ``max_tokens`` is refused: its table row and length stay, its tokens
+    get slot -1. So is the first one that the free stack cannot serve, and every later one that needs a block. All
+    tensors are contiguous int32 CUDA tensors (at most 8192 sequences), read on the GPU and trusted; free_blocks and
+    free_count are not changed - give the returned count to the next call. No counterpart in the reference."""
+    call, b, width = _table_operands(block_table, page, lens=lens, new_lens=new_lens, free_blocks=free_blocks,
+                                     free_count=free_count)
+    if int(max_tokens) != max_tokens or not 0 <= max_tokens <= 0x7fffffff:
+        raise ValueError(f"max_tokens {max_tokens}: a count of tokens below 2^31 is expected")
+    slots, starts, lens_out, left = (call.new((k,)) for k in (int(max_tokens), b + 1, b, 1))
+    call.launch(_fusedtok.block_table_extend_launch, block_table.data_ptr(), lens.data_ptr(), new_lens.data_ptr(),
+                free_blocks.data_ptr(), free_count.data_ptr(), slots.data_ptr(), starts.data_ptr(),
+                lens_out.data_ptr(), left.data_ptr(), b, width, int(page), free_blocks.shape[0], int(max_tokens))
+    return BlockTableStep(slots, starts, lens_out, left)
+
+
+def block_table_trim(block_table, lens, keep_lens, free_blocks, free_count, page):
+    """Cut sequences back to ``min(lens[b], keep_lens[b])`` tokens (0: finished, or a shorter length: rejected draft
+    tokens) and push the blocks that they no longer need on the free stack, in batch order, from
+    ``free_blocks[free_count]`` on. Returns ``(lens, free_count)``, the new lengths and count; the table is only read.
+    Operands as in :func:`block_table_extend`. No counterpart in the reference."""
+    call, b, width = _table_operands(block_table, page, lens=lens, keep_lens=keep_lens, free_blocks=free_blocks,
+                                     free_count=free_count)
+    lens_out, left = call.new((b,)), call.new((1,))
+    call.launch(_fusedtok.block_table_trim_launch, block_table.data_ptr(), lens.data_ptr(), keep_lens.data_ptr(),
+                free_blocks.data_ptr(), free_count.data_ptr(), lens_out.data_ptr(), left.data_ptr(), b, width,
+                int(page), free_blocks.shape[0])
+    return lens_out, left

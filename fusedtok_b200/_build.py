@@ -1,56 +1,100 @@
 """In-tree build of the CUDA library (sm_100a only).
 
-``python fusedtok_b200/_build.py`` compiles ``csrc/fusedtok_b200.cu`` into
+``python fusedtok_b200/_build.py`` compiles ``csrc/*.cu`` into
 ``fusedtok_b200/libfusedtok_b200.so`` with nvcc. The library is the whole
 product: there is no other backend and no CPU fallback, so importing the
 package without it fails.
 """
 
 import os
+import re
 import subprocess
 import sys
+import time
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libfusedtok_b200.so")
-SOURCES = ["fusedtok_b200.cu"]
-HEADERS = sorted(f for f in os.listdir(CSRC) if f.endswith(".cuh")) + [
-    os.path.join("..", "..", "include", "fusedtok_b200.h")]
+SOURCES = sorted(f for f in os.listdir(CSRC) if f.endswith(".cu"))
+OBJECTS = os.path.join(HERE, "build")       # one object per source and variant, kept between builds
 
 NVCC_FLAGS = [
     "-O3", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
-    "-Xcompiler", "-fPIC", "-shared", "-cudart", "static",
+    "-Xcompiler", "-fPIC",
 ]
+LINK_FLAGS = ["-shared", "-cudart", "static", "-gencode", "arch=compute_100a,code=sm_100a"]
 
 
 # The self-checking variant (tests/test_bounds_build_gpu.py): same sources with -DFTK_BOUNDS.
 BOUNDS_LIB = os.path.join(HERE, "libfusedtok_b200_bounds.so")
 
 
-def stale(target=None):
-    target = target or LIB
+def _includes(path, seen=None):
+    """`path` and every file it includes with quotes, directly or not."""
+    seen = set() if seen is None else seen
+    path = os.path.normpath(path)
+    if path in seen or not os.path.exists(path):
+        return seen
+    seen.add(path)
+    with open(path) as f:
+        for name in re.findall(r'^\s*#include "([^"]+)"', f.read(), flags=re.M):
+            _includes(os.path.join(os.path.dirname(path), name), seen)
+    return seen
+
+
+def _out_of_date(target, source):
     if not os.path.exists(target):
         return True
     t = os.path.getmtime(target)
-    deps = [os.path.join(CSRC, f) for f in SOURCES + HEADERS]
-    return any(os.path.exists(d) and os.path.getmtime(d) > t for d in deps)
+    return any(os.path.getmtime(d) > t for d in _includes(source))
 
 
-def _command(defines, target, verbose=False):
-    cmd = ["nvcc"] + NVCC_FLAGS + ["-D" + d for d in defines]
-    if verbose:
-        cmd += ["-Xptxas", "-v"]
-    return cmd + [os.path.join(CSRC, s) for s in SOURCES] + ["-o", target]
+def stale(target=None):
+    target = target or LIB
+    return any(_out_of_date(target, os.path.join(CSRC, s)) for s in SOURCES)
+
+
+def _compile(variants, force=False, verbose=False):
+    """Bring the objects of `variants` [(defines, target)] up to date, every source in an nvcc of its own side by
+    side, and link each variant's library. What is built is dated from when the build began: an edit made meanwhile
+    leaves it out of date."""
+    os.makedirs(OBJECTS, exist_ok=True)
+    began = time.time()
+    jobs, linked = [], []
+    for defines, target in variants:
+        tag = "".join("_" + re.sub(r"\W", "_", d) for d in sorted(defines))
+        objects = []
+        for s in SOURCES:
+            source, obj = os.path.join(CSRC, s), os.path.join(OBJECTS, s[:-3] + tag + ".o")
+            objects.append(obj)
+            if force or _out_of_date(obj, source):
+                jobs.append((os.path.getsize(source), ["nvcc"] + NVCC_FLAGS + ["-D" + d for d in defines]
+                             + (["-Xptxas", "-v"] if verbose else []) + ["-c", source, "-o", obj]))
+        linked.append((objects, target))
+    jobs.sort(key=lambda j: -j[0])                    # the longest first
+    running, failed = [], []
+    while jobs or running:
+        while jobs and len(running) < max(2, os.cpu_count() or 2):
+            cmd = jobs.pop(0)[1]
+            running.append((cmd, subprocess.Popen(cmd)))
+        cmd, job = running.pop(0)
+        try:
+            if job.wait(timeout=1) != 0:
+                failed.append(cmd[-1])
+            else:
+                os.utime(cmd[-1], (began, began))
+        except subprocess.TimeoutExpired:
+            running.append((cmd, job))
+    if failed:
+        raise RuntimeError("nvcc failed for " + ", ".join(failed))
+    for objects, target in linked:
+        subprocess.check_call(["nvcc"] + LINK_FLAGS + objects + ["-o", target])
+        os.utime(target, (began, began))
 
 
 def build_all(force=False):
-    """The product and the self-checking variant, whichever is out of date, compiled side by side (each
-    is one long nvcc run)."""
-    jobs = [(t, subprocess.Popen(_command(d, t))) for d, t in (((), LIB), (("FTK_BOUNDS",), BOUNDS_LIB))
-            if force or stale(t)]
-    failed = [t for t, job in jobs if job.wait() != 0]
-    if failed:
-        raise RuntimeError("nvcc failed for " + ", ".join(failed))
+    """The product and the self-checking variant, whichever is out of date, compiled side by side."""
+    _compile([(d, t) for d, t in (((), LIB), (("FTK_BOUNDS",), BOUNDS_LIB)) if force or stale(t)], force)
     return LIB
 
 
@@ -61,7 +105,7 @@ def build(force=False, verbose=False, defines=(), out=None):
     target = out or LIB
     if not force and not defines and not stale():
         return LIB
-    subprocess.check_call(_command(defines, target, verbose))
+    _compile([(tuple(defines), target)], force, verbose)
     return target
 
 

@@ -65,6 +65,13 @@ _lib.fusedtok_exchange_open.argtypes = [ctypes.c_char_p, ctypes.POINTER(_vp)]
 _lib.fusedtok_exchange_close.argtypes = [_vp]
 _lib.fusedtok_attention_decode_exchange_launch.argtypes = (
     [_i] + [_vp] * 5 + [ctypes.POINTER(_vp)] + [_i] * 7 + [_sz])
+_lib.fusedtok_attention_decode_paged_q8_workspace.argtypes = [_i] * 7
+_lib.fusedtok_attention_decode_paged_q8_workspace.restype = ctypes.c_longlong
+_lib.fusedtok_attention_decode_paged_q8_launch.argtypes = (
+    [_i] * 2 + [_vp] * 8 + [ctypes.c_longlong] + [_i] * 5 + [ctypes.c_longlong, _i, _sz])
+_lib.fusedtok_kv_append_paged_q8_launch.argtypes = [_i] * 2 + [_vp] * 6 + [_i] * 4 + [ctypes.c_longlong, _sz]
+_lib.fusedtok_block_table_extend_launch.argtypes = [_vp] * 9 + [_i] * 5 + [_sz]
+_lib.fusedtok_block_table_trim_launch.argtypes = [_vp] * 7 + [_i] * 4 + [_sz]
 _lib.fusedtok_attention_device_status.argtypes = [ctypes.POINTER(_i)]
 _lib.fusedtok_attention_launch_count.argtypes = [_i]
 _lib.fusedtok_attention_launch_count.restype = ctypes.c_longlong
@@ -94,6 +101,8 @@ EXPORTS = (
     "fusedtok_exchange_alloc", "fusedtok_exchange_free", "fusedtok_exchange_export",
     "fusedtok_exchange_open", "fusedtok_exchange_close", "fusedtok_attention_decode_exchange_launch",
     "fusedtok_attention_decode_launch_noalloc",
+    "fusedtok_attention_decode_paged_q8_workspace", "fusedtok_attention_decode_paged_q8_launch",
+    "fusedtok_kv_append_paged_q8_launch", "fusedtok_block_table_extend_launch", "fusedtok_block_table_trim_launch",
     "fusedtok_attention_device_status", "fusedtok_attention_launch_count", "fusedtok_debug_poke_status",
     "fusedtok_debug_set_pool_blocks", "fusedtok_debug_read_stream",
 )
@@ -388,6 +397,46 @@ def attention_decode_launch_noalloc(dtype, q, k, v, lens, out, batch, hq, hkv, t
     on a device outside stream capture; do not overlap calls on one device."""
     _check(_lib.fusedtok_attention_decode_launch_noalloc(
         dtype, int(q), int(k), int(v), _opt(lens), int(out), batch, hq, hkv, t_seq, dim, int(stream)))
+
+
+def attention_decode_paged_q8_workspace(dtype, batch, hq, hkv, page, tbl_width, dim):
+    """Bytes of workspace a call of attention_decode_paged_q8_launch with these shapes needs on the current device."""
+    n = _lib.fusedtok_attention_decode_paged_q8_workspace(dtype, batch, hq, hkv, page, tbl_width, dim)
+    if n < 0:
+        _check(-n)
+    return n
+
+
+def attention_decode_paged_q8_launch(dtype, store, q, k_pool, v_pool, kv_scales, table, lens, out, workspace,
+                                     workspace_bytes, batch, hq, hkv, page, tbl_width, num_blocks, dim, stream=0):
+    """Decode attention over a paged cache of one-byte codes with a scale per (block, kv head). dtype (q, out):
+    0 float32, 1 bfloat16, 2 float16; store: 0 int8, 1 e4m3. The workspace belongs to the call until it is done."""
+    _check(_lib.fusedtok_attention_decode_paged_q8_launch(
+        dtype, store, q, k_pool, v_pool, kv_scales, table, _opt(lens), out, _opt(workspace), workspace_bytes, batch,
+        hq, hkv, page, tbl_width, num_blocks, dim, stream))
+
+
+def kv_append_paged_q8_launch(dtype, store, k_new, v_new, slots, k_pool, v_pool, kv_scales, tokens, hkv, dim, page,
+                              num_blocks, stream=0):
+    """Round `tokens` new K and V rows into the 8-bit paged cache at their slots (block * page + offset; a slot
+    outside the pool passes its token over)."""
+    _check(_lib.fusedtok_kv_append_paged_q8_launch(dtype, store, k_new, v_new, slots, k_pool, v_pool, kv_scales,
+                                                   tokens, hkv, dim, page, num_blocks, stream))
+
+
+def block_table_extend_launch(table, lens, new_lens, free_blocks, free_count, slots, starts, lens_out, free_count_out,
+                              batch, tbl_width, page, free_capacity, max_tokens, stream=0):
+    """Blocks for new_lens[b] more tokens of each sequence off the free stack, and the slot of every new token."""
+    _check(_lib.fusedtok_block_table_extend_launch(table, lens, new_lens, free_blocks, free_count, slots, starts,
+                                                   lens_out, free_count_out, batch, tbl_width, page, free_capacity,
+                                                   max_tokens, stream))
+
+
+def block_table_trim_launch(table, lens, keep_lens, free_blocks, free_count, lens_out, free_count_out, batch,
+                            tbl_width, page, free_capacity, stream=0):
+    """Cut sequences back to keep_lens[b] tokens and push the blocks no longer needed on the free stack."""
+    _check(_lib.fusedtok_block_table_trim_launch(table, lens, keep_lens, free_blocks, free_count, lens_out,
+                                                 free_count_out, batch, tbl_width, page, free_capacity, stream))
 
 
 def attention_device_status():

@@ -1,0 +1,832 @@
+// Decode attention over a paged cache held in 8 bits (int8 or e4m3 codes) with one scale per (block, kv head)
+// for K and one for V: out = softmax_t(ks[t] * q . k8_t / sqrt(D)) . (vs[t] * v8_t).
+//
+// What bounds it: HBM. A cache row is 2 * D bytes for 4 * G * D flops (G query heads per kv head). Half the bytes of a
+// 16-bit cache for the same arithmetic, so the conversions count: every code becomes a half exactly once, in
+// registers, on its way from shared memory to the tensor cores. Both code types are exact in half precision, and
+// the scales never touch the codes: ks multiplies the finished score, vs is folded into the softmax weight.
+//
+// Structure (see decode_tc.cuh for the parts both share): one persistent CTA per SM, 1 producer warp that streams
+// 64-row tiles with TMA into a ring in shared memory, 8 consumer warps; all tiles of all units cut at equal cost
+// into one range per CTA, worked out on the device from lens.
+//  * Stage layout: a block's (page x D) bytes are contiguous in the pool, so the pool is described to TMA as 128-byte
+//    lines with the 128-byte swizzle, whatever D is; row r, 16-byte chunk c of a tile sits at line-linear address
+//    r * D + 16 c, swizzled. One copy per block and tile for K, one for V; the two scales of the block follow with an
+//    8-byte cp.async that signals the same mbarrier.
+//  * K and V are the A operand of mma.m16n8k16 (rows / head dim on M, query heads on N). ldmatrix moves 16-bit units,
+//    i.e. pairs of codes: for K the pair is two neighbouring d, the order of d inside a 16-step is permuted and the
+//    query fragments are loaded in that same order; for V^T (transposing load) the pair is two neighbouring d of one
+//    row, the byte permutation that widens the codes also splits them, and a 16-row block of O^T holds the even d in
+//    its upper half and the odd d in its lower half.
+//  * Weights: with |vs| = c * 2^e, 1 <= c < 2, the running maximum R is that of s + e (log2 units) and the weight
+//    w = 2^(s + e - R) lies in [0, 1]: the MMA gets w * c, rounded to half relative to the largest CONTRIBUTION so far, and
+//    l += w * 2^-e, the sum of 2^(s - R), stays in fp32. e is counted from a warp's first block, so that both stay in
+//    range as long as the V scales of a sequence differ by less than 2^60; scales below 2^-126 count as 0.
+//  * SPLIT: with at most 4 query heads per unit (8 with two column blocks) each head takes two of the 8 MMA columns, the
+//    value rounded to half and the remainder: q and P' then carry 22 bits at no cost in MMAs. float32 calls always run
+//    this way (that is what keeps them at float32 accuracy on half-precision tensor cores), 16-bit calls when their
+//    heads fit.
+//  * A unit that lies in one range is finished in place. Otherwise the CTAs leave (m, l, acc) partials, at most two per
+//    range, in a workspace that belongs to the call, and q8_merge_kernel, launched behind with programmatic stream
+//    serialization, folds them in range order. No counters, no state between calls: calls on different streams, and
+//    captured graphs, cannot meet in it.
+// Every mbarrier wait is bounded (2 s); on expiry the kernel records a status code and runs to completion.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "decode_tc.cuh"
+
+namespace ftk {
+
+constexpr int Q8_WPT = 2;                       // consumer warps per tile
+constexpr int Q8_NG = NCW / Q8_WPT;             // groups of warps, taking tiles in turn
+constexpr int Q8_RB = 4 / Q8_WPT;               // 16-row blocks of a tile per warp
+constexpr int Q8_MAX_SPLIT = 32;                // generic kernel: most ranges a unit is cut into
+
+struct Q8Params : DecodeParams {
+    const float2* scales;      // [blocks][Hkv] (K, V)
+    long long blocks;          // blocks of the pool
+    int4* desc;                // [ncta] unit whose merge starts in this range: (b, unit of b, partials, -)
+    int out_dt;                // type of q and out: 0 float32, 1 bfloat16, 2 float16
+    int nsplit;                // generic kernel: ranges per unit
+};
+
+// q and out carry their type at run time: only the first and last step of a unit look at it.
+struct AnyOut {};
+__device__ __forceinline__ float4 load4_any(const void* base, size_t at, int dt) {
+    if (dt == 0) return Store<float>::ld4(static_cast<const float*>(base) + at);
+    if (dt == 1) return Store<__nv_bfloat16>::ld4(static_cast<const __nv_bfloat16*>(base) + at);
+    return Store<__half>::ld4(static_cast<const __half*>(base) + at);
+}
+__device__ __forceinline__ void store4_any(void* base, size_t at, int dt, float4 v) {
+    if (dt == 0) Store<float>::st4(static_cast<float*>(base) + at, v);
+    else if (dt == 1) Store<__nv_bfloat16>::st4(static_cast<__nv_bfloat16*>(base) + at, v);
+    else Store<__half>::st4(static_cast<__half*>(base) + at, v);
+}
+__device__ __forceinline__ void store2_any(void* base, size_t at, int dt, float a, float b) {
+    if (dt == 0) Store<float>::st2(static_cast<float*>(base) + at, a, b);
+    else if (dt == 1) Store<__nv_bfloat16>::st2(static_cast<__nv_bfloat16*>(base) + at, a, b);
+    else Store<__half>::st2(static_cast<__half*>(base) + at, a, b);
+}
+template <> __device__ inline void zero_rows<AnyOut>(const DecodeParams& p, int b, unsigned int) {
+    const int dt = static_cast<const Q8Params&>(p).out_dt;
+    const int n = p.Hq * p.D;
+    for (int i = 0; i < n; i += 4) store4_any(p.out, (size_t)b * n + i, dt, make_float4(0.f, 0.f, 0.f, 0.f));
+}
+
+// ---- 8-bit codes to half pairs -------------------------------------------------
+// `pairs`: bytes (0, 1) and (2, 3) of a word; `crossed`: bytes (0, 2) and (1, 3).
+template <typename KV> struct Codes;
+template <> struct Codes<int8_t> {
+    // byte u = code + 128 as the low mantissa bits of 1024 (0x6400 | u is the half 1024 + u), less 1152: exact
+    static __device__ __forceinline__ uint32_t off(uint32_t x) {
+        const __half2 v = __hsub2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    static __device__ __forceinline__ void pairs(uint32_t r, uint32_t& a, uint32_t& b) {
+        const uint32_t u = r ^ 0x80808080u;
+        a = off(__byte_perm(u, 0x64646464u, 0x4140));
+        b = off(__byte_perm(u, 0x64646464u, 0x4342));
+    }
+    static __device__ __forceinline__ void crossed(uint32_t r, uint32_t& a, uint32_t& b) {
+        const uint32_t u = r ^ 0x80808080u;
+        a = off(__byte_perm(u, 0x64646464u, 0x4240));
+        b = off(__byte_perm(u, 0x64646464u, 0x4341));
+    }
+    static __device__ __forceinline__ float4 floats(uint32_t r) {
+        return make_float4((float)(int8_t)(r & 255u), (float)(int8_t)((r >> 8) & 255u), (float)(int8_t)((r >> 16) & 255u),
+                           (float)(int8_t)(r >> 24));
+    }
+};
+template <> struct Codes<__nv_fp8_e4m3> {
+    static __device__ __forceinline__ void pairs(uint32_t r, uint32_t& a, uint32_t& b) {
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+            : "=r"(a), "=r"(b) : "r"(r));
+    }
+    static __device__ __forceinline__ void crossed(uint32_t r, uint32_t& a, uint32_t& b) {
+        pairs(__byte_perm(r, r, 0x3120), a, b);
+    }
+    static __device__ __forceinline__ float4 floats(uint32_t r) {
+        uint32_t a, b;
+        pairs(r, a, b);
+        const float2 lo = __half22float2(*reinterpret_cast<__half2*>(&a)), hi = __half22float2(*reinterpret_cast<__half2*>(&b));
+        return make_float4(lo.x, lo.y, hi.x, hi.y);
+    }
+};
+
+template <int D> struct Q8Cfg {
+    static_assert(D % 16 == 0 && D >= 64 && D <= 256, "head dim: a multiple of 16 from 64 to 256");
+    static constexpr int KV_BYTES = TILE * D;          // a multiple of 1024: the swizzle phase of every stage is the same
+    static constexpr int STAGE_BYTES = 2 * KV_BYTES;
+    // 128 KB of tiles in flight per SM, as in the 16-bit kernel; a multiple of the number of groups, so that a stage is
+    // always consumed by the same group, which then sees every phase of its barrier in order
+    static constexpr int NS = (131072 / STAGE_BYTES) / Q8_NG * Q8_NG;
+    static_assert(NS >= Q8_NG, "ring shorter than the groups");
+    static constexpr int ACC_STRIDE = D + 4;
+    static constexpr int SCRATCH_BYTES = NCW * 8 * ACC_STRIDE * 4;
+    static constexpr int OFF_SCRATCH = NS * STAGE_BYTES;
+    static constexpr int OFF_ML = OFF_SCRATCH + SCRATCH_BYTES;       // [NCW][8] (m, l)
+    static constexpr int OFF_SCALE = OFF_ML + NCW * 8 * 8;           // [NS][4] (K, V) scales of the stage's blocks
+    static constexpr int OFF_BAR = OFF_SCALE + NS * 4 * 8;           // full[NS], empty[NS]
+    static constexpr int OFF_SCHED = OFF_BAR + 2 * NS * 8;
+    static constexpr int OFF_ABORT = OFF_SCHED + (int)sizeof(SchedShared);
+    static constexpr int OFF_PREFIX = (OFF_ABORT + 16 + 15) & ~15;
+    static constexpr int OFF_ZPRE = OFF_PREFIX + (SCHED_MAX_B + 1) * 4;
+    static constexpr int SMEM_BYTES = OFF_ZPRE + (SCHED_MAX_B + 1) * 4 + 8;
+    static_assert(SMEM_BYTES <= 232448, "exceeds the 227 KB of shared memory a CTA can have");
+};
+
+__device__ __forceinline__ void tma_load_lines(uint32_t dst, const CUtensorMap* map, int line, uint32_t bar, uint64_t pol) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%2, %3}], [%4], %5;"
+        ::"r"(dst), "l"(map), "r"(0), "r"(line), "r"(bar), "l"(pol)
+        : "memory");
+}
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+// this thread's arrival on `bar`, made when its cp.async copies so far have landed
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// Powers of two f, g with f * g = 1 and |x| * f in [1, 2) for a row's largest magnitude x (NaN for a row that is not finite).
+__device__ __forceinline__ void row_exponent(float x, float& f, float& g) {
+    const unsigned int e = (__float_as_uint(x) >> 23) & 255u;
+    f = e == 254u ? __uint_as_float(0x00400000u) : __uint_as_float((254u - e) << 23);
+    g = e == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(e << 23);
+    if (e == 255u) f = __uint_as_float(0x7fc00000u);
+}
+
+// ---- the kernel ----------------------------------------------------------------
+// KV: code type. NBK: 8-column blocks of the MMA. SPLIT: two columns per query head (see above).
+template <typename KV, int D, int NBK, bool SPLIT>
+__global__ void __launch_bounds__(TC_THREADS, 1)
+decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Q8Params p) {
+    using Cfg = Q8Cfg<D>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    SchedShared* sh = reinterpret_cast<SchedShared*>(smem + Cfg::OFF_SCHED);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Cfg::OFF_ABORT);
+    const uint32_t smem_base = smem_u32(smem);
+    const uint32_t bar_full = smem_base + Cfg::OFF_BAR;
+    const uint32_t bar_empty = bar_full + Cfg::NS * 8;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int cta = (int)blockIdx.x;
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        if (smem_base & 1023u) {
+            *abort_flag = 1;
+            atomicCAS(p.status, ST_OK, ST_SMEM_MISALIGNED);
+        }
+        for (int s = 0; s < Cfg::NS; ++s) {
+            mbar_init(bar_full + s * 8, 33);           // the announced bytes, and each producer lane's scales
+            mbar_init(bar_empty + s * 8, Q8_WPT);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_k) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_v) : "memory");
+    }
+    __syncthreads();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int upb = p.Hkv * p.NCH;
+    const unsigned int* prefix = nullptr;
+    const unsigned int* zprefix = nullptr;
+    long long total;
+    Plan pl;
+    if (!p.lens) {
+        total = (long long)p.B * tiles_of(p.T) * upb;
+        pl = make_plan(total, p.ncta, 0, 0);
+        if (total > 0) plan_enable_cost(pl, (long long)p.B * tiles_of(p.T), p.B, upb, nullptr, nullptr, tiles_of(p.T), 1, 1);
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+    } else {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        unsigned int* table = reinterpret_cast<unsigned int*>(smem + Cfg::OFF_PREFIX);
+        unsigned int* ztable = reinterpret_cast<unsigned int*>(smem + Cfg::OFF_ZPRE);
+        total = sched_prefix<AnyOut>(p, sh, table, ztable, 0);
+        prefix = table;
+        zprefix = ztable;
+        pl = make_plan(total, p.ncta, 0, 0);
+        if (total > 0) plan_enable_cost(pl, prefix[p.B], zprefix[p.B], upb, prefix, zprefix, 0, 1, 1);
+    }
+    if (*abort_flag) {
+        if (threadIdx.x == 0) p.desc[cta] = make_int4(0, 0, 0, 0);
+        return;
+    }
+    // every warp locates the CTA's range for itself
+    Walker w = {};
+    if (total > 0) {
+        if (pl.ctot) w = walker_locate_cost_range(p, pl, cta);
+        else if (!range_empty(pl, cta)) w = walker_locate(p, prefix, range_start(pl, cta), range_start(pl, cta + 1));
+    }
+
+    if (warp == NCW) {
+        // ===================== producer warp =====================
+        const uint64_t pol = policy_evict_first();
+        const int* tbl = nullptr;
+        int issued = 0, s = 0;
+        uint32_t ph = 0;
+        // 32 consecutive table entries of the current sequence, one per lane, and the 32 behind them, already on their way
+        int tbl_b = -1, tbl_base = 0, tbl_val = 0, tbl_next = 0;
+        bool gave_up = false;
+        while (w.g < w.end) {
+            const int kv = w.ub / p.NCH;
+            const int t0 = w.ti * TILE;
+            const int pg0 = p.page <= TILE ? t0 >> p.box_shift : t0 / p.page;
+            const int npg = p.page <= TILE ? (min(TILE, w.len - t0) + p.page - 1) >> p.box_shift : 1;
+            if (tbl_b != w.b || pg0 < tbl_base || pg0 + npg > tbl_base + 32) {
+                tbl = p.table + (size_t)w.b * p.tbl_width;
+                if (tbl_b == w.b && pg0 == tbl_base + 32) {
+                    tbl_val = tbl_next;
+                } else {
+                    tbl_val = pg0 + lane < p.tbl_width ? __ldg(tbl + pg0 + lane) : 0;
+                }
+                tbl_base = pg0;
+                tbl_b = w.b;
+                tbl_next = pg0 + 32 + lane < p.tbl_width ? __ldg(tbl + pg0 + 32 + lane) : 0;
+            }
+            int blk = __shfl_sync(0xffffffffu, tbl_val, (pg0 - tbl_base + lane) & 31);
+            if (lane < npg && !(blk >= 0 && blk < p.blocks)) blk = 0;      // (device table values are trusted: address only)
+            const long long unit_row = ((long long)blk * p.Hkv + kv) * p.page + (p.page <= TILE ? 0 : t0 - pg0 * p.page);
+            const int line = (int)(unit_row * D >> 7);
+            const uint32_t bytes = (uint32_t)(npg << p.box_shift) * (uint32_t)(2 * D);
+            if (!mbar_wait(bar_empty + s * 8, ph ^ 1u, abort_flag, p.status, ST_WAIT_EMPTY_TIMEOUT)) {
+                gave_up = true;
+                break;
+            }
+            const uint32_t fb = bar_full + s * 8;
+            if (lane == 0) mbar_expect_tx(fb, bytes);
+            __syncwarp();                                                   // expect_tx before any complete_tx
+            if (lane < npg) {
+                const uint32_t dst = smem_base + s * Cfg::STAGE_BYTES + (uint32_t)(lane << p.box_shift) * (uint32_t)D;
+                tma_load_lines(dst, &tm_k, line, fb, pol);
+                tma_load_lines(dst + Cfg::KV_BYTES, &tm_v, line, fb, pol);
+                cp_async8(smem_base + Cfg::OFF_SCALE + (s * 4 + lane) * 8, p.scales + (size_t)blk * p.Hkv + kv);
+            }
+            cp_async_arrive(fb);
+            ++issued;
+            walker_advance(p, w);
+            if (++s == Cfg::NS) { s = 0; ph ^= 1u; }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        if (gave_up || *abort_flag) {
+            // do not leave the CTA while its own copies may still be landing: wait (bounded) for every stage issued
+            const int first = issued > Cfg::NS ? issued - Cfg::NS : 0;
+            for (int i = first; i < issued; ++i) {
+                const unsigned long long b0 = global_ns();
+                while (!mbar_try_wait(bar_full + (i % Cfg::NS) * 8, (uint32_t)((i / Cfg::NS) & 1))) {
+                    if (global_ns() - b0 > WAIT_LIMIT_NS) {
+                        atomicCAS(p.status, ST_OK, ST_DRAIN_TIMEOUT);
+                        break;
+                    }
+                }
+            }
+        }
+        return;
+    }
+
+    // ======================= consumer warps =======================
+    const int cg = warp / Q8_WPT, wr = warp % Q8_WPT;
+    const int quad = lane >> 2, qi = lane & 3;
+    const int tc = threadIdx.x;
+    const float neg_inf = -INFINITY;
+    float* s_acc = reinterpret_cast<float*>(smem + Cfg::OFF_SCRATCH);
+    float2* s_ml = reinterpret_cast<float2*>(smem + Cfg::OFF_ML);
+
+    constexpr int KSTEPS = D / 16;
+    constexpr int NLD = (KSTEPS + 1) / 2;          // ldmatrix.x4 per 16 rows: two 16-byte chunks of 16 rows
+    constexpr int HB = SPLIT ? 4 : 8;              // query heads per column block
+    constexpr int HPT = SPLIT ? 1 : 2;             // of which this thread holds the scores of
+    uint32_t qb[NBK][KSTEPS][2];
+    float acc[NBK][KSTEPS][4];                     // O^T block mt: d = 16 mt + 2 quad ([0], [1]) and + 1 ([2], [3])
+    float kf[NBK][HPT];                            // score factor of the head: its row's exponent / sqrt(D) * log2(e)
+    float m_run[NBK][HPT], l_run[NBK][HPT];        // R of the head; this thread's share of l
+    int e0 = -1;                                   // biased exponent that this warp counts V scales from
+
+    // Byte offset of chunk 2 i + csel of row r inside a tile, swizzled. `csel` and the row are the lane's.
+    const int lrow = ((lane >> 3) & 1) * 8 + (lane & 7), csel = lane >> 4;
+    auto chunk_off = [&](int j, int i) -> uint32_t {
+        const uint32_t lin = (uint32_t)((wr * Q8_RB + j) * 16 + lrow) * (uint32_t)D + (uint32_t)(2 * i + csel) * 16u;
+        return lin ^ (((lin >> 7) & 7u) << 4);
+    };
+
+    int i0 = 0, own = cg, s = cg;
+    uint32_t ph = 0;
+
+    auto process = [&](auto ragged_tag, int rows_valid) {
+        constexpr bool RAGGED = decltype(ragged_tag)::value;
+        const uint32_t st_k = smem_base + s * Cfg::STAGE_BYTES;
+        const uint32_t st_v = st_k + Cfg::KV_BYTES;
+        const float2* sc = reinterpret_cast<const float2*>(smem + Cfg::OFF_SCALE) + s * 4;
+        float2 ks[Q8_RB];
+#pragma unroll
+        for (int j = 0; j < Q8_RB; ++j) {
+            const int r0 = (wr * Q8_RB + j) * 16;
+            ks[j] = sc[r0 >> p.box_shift];
+            // a block of the tile that holds no valid row was not copied, nor were its scales
+            if (RAGGED && r0 >= rows_valid) ks[j] = make_float2(0.0f, 0.0f);
+        }
+        constexpr int PF = 2;
+        constexpr int N = Q8_RB * NLD;
+        uint32_t f[PF][4];
+        // ---- S^T = K Q^T
+        float sa[NBK][Q8_RB][4];
+#pragma unroll
+        for (int nbk = 0; nbk < NBK; ++nbk)
+#pragma unroll
+            for (int j = 0; j < Q8_RB; ++j) sa[nbk][j][0] = sa[nbk][j][1] = sa[nbk][j][2] = sa[nbk][j][3] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < PF; ++n) ldsm_x4(st_k + chunk_off(n / NLD, n % NLD), f[n][0], f[n][1], f[n][2], f[n][3]);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int j = n / NLD, i = n % NLD;
+            uint32_t (&r)[4] = f[n % PF];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int kk = 2 * i + half;
+                if (kk < KSTEPS) {
+                    uint32_t a0, a1, a2, a3;
+                    Codes<KV>::pairs(r[2 * half], a0, a2);
+                    Codes<KV>::pairs(r[2 * half + 1], a1, a3);
+#pragma unroll
+                    for (int nbk = 0; nbk < NBK; ++nbk)
+                        mma16816<__half>(sa[nbk][j], a0, a1, a2, a3, qb[nbk][kk][0], qb[nbk][kk][1]);
+                }
+            }
+            if (n + PF < N) ldsm_x4(st_k + chunk_off((n + PF) / NLD, (n + PF) % NLD), r[0], r[1], r[2], r[3]);
+        }
+#pragma unroll
+        for (int n = 0; n < PF; ++n) ldsm_x4_t(st_v + chunk_off(n / NLD, n % NLD), f[n][0], f[n][1], f[n][2], f[n][3]);
+        // ---- online softmax, in units of log2
+        if (e0 < 0) e0 = (int)min(max((__float_as_uint(ks[0].y) >> 23) & 255u, 64u), 190u);
+        float de[Q8_RB], ge[Q8_RB], ce[Q8_RB];    // per block: exponent of vs less e0, 2^-that, and what is left of vs
+#pragma unroll
+        for (int j = 0; j < Q8_RB; ++j) {
+            const int d = min(max((int)((__float_as_uint(ks[j].y) >> 23) & 255u) - e0, -60), 60);
+            de[j] = (float)d;
+            ge[j] = __uint_as_float((uint32_t)(127 - d) << 23);
+            ce[j] = ks[j].y * __uint_as_float((uint32_t)(254 - (e0 + d)) << 23);
+        }
+        uint32_t pb[NBK][Q8_RB][2];
+#pragma unroll
+        for (int nbk = 0; nbk < NBK; ++nbk) {
+            float pw[HPT][Q8_RB][2];
+#pragma unroll
+            for (int e = 0; e < HPT; ++e) {
+                float v[Q8_RB][2];
+                float mx = neg_inf;
+#pragma unroll
+                for (int j = 0; j < Q8_RB; ++j) {
+                    const float fac = kf[nbk][e] * ks[j].x;
+                    const int r_lo = (wr * Q8_RB + j) * 16 + quad;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        v[j][h] = fmaf(SPLIT ? sa[nbk][j][2 * h] + sa[nbk][j][2 * h + 1] : sa[nbk][j][2 * h + e], fac, de[j]);
+                        if (RAGGED && r_lo + 8 * h >= rows_valid) v[j][h] = neg_inf;
+                        mx = fmaxf(mx, v[j][h]);
+                    }
+                }
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                const float m_old = m_run[nbk][e];
+                const float m_new = fmaxf(m_old, mx);
+                const float m_safe = m_new == neg_inf ? 0.0f : m_new;
+                float sum = 0.0f;
+#pragma unroll
+                for (int j = 0; j < Q8_RB; ++j)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float w8 = ex2(v[j][h] - m_safe);
+                        sum = fmaf(w8, ge[j], sum);
+                        pw[e][j][h] = w8 * ce[j];
+                    }
+                if (m_new != m_old) {
+                    const float alpha = ex2(m_old - m_safe);
+                    m_run[nbk][e] = m_new;
+                    l_run[nbk][e] *= alpha;
+#pragma unroll
+                    for (int mt = 0; mt < KSTEPS; ++mt) {
+                        if constexpr (SPLIT) {
+                            acc[nbk][mt][0] *= alpha; acc[nbk][mt][1] *= alpha;
+                            acc[nbk][mt][2] *= alpha; acc[nbk][mt][3] *= alpha;
+                        } else {
+                            acc[nbk][mt][e] *= alpha;
+                            acc[nbk][mt][2 + e] *= alpha;
+                        }
+                    }
+                }
+                l_run[nbk][e] += sum;
+            }
+#pragma unroll
+            for (int j = 0; j < Q8_RB; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if constexpr (SPLIT) {
+                        const float hi = __half2float(__float2half_rn(pw[0][j][h]));
+                        pb[nbk][j][h] = movmatrix_trans(pack2<__half>(hi, pw[0][j][h] - hi));
+                    } else {
+                        pb[nbk][j][h] = movmatrix_trans(pack2<__half>(pw[0][j][h], pw[HPT - 1][j][h]));
+                    }
+                }
+        }
+        // ---- O^T += V^T P^T
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int j = n / NLD, i = n % NLD;
+            uint32_t (&r)[4] = f[n % PF];
+            if constexpr (RAGGED) {
+                // rows at and past the end may hold anything, NaN codes included: a zero weight times them has to be zero
+                const int t = (wr * Q8_RB + j) * 16 + qi * 2;
+                const uint32_t lo = (t < rows_valid ? 0x0000ffffu : 0u) | (t + 1 < rows_valid ? 0xffff0000u : 0u);
+                const uint32_t hi = (t + 8 < rows_valid ? 0x0000ffffu : 0u) | (t + 9 < rows_valid ? 0xffff0000u : 0u);
+                r[0] &= lo; r[1] &= hi; r[2] &= lo; r[3] &= hi;
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int mt = 2 * i + half;
+                if (mt < KSTEPS) {
+                    uint32_t a0, a1, a2, a3;
+                    Codes<KV>::crossed(r[2 * half], a0, a1);
+                    Codes<KV>::crossed(r[2 * half + 1], a2, a3);
+#pragma unroll
+                    for (int nbk = 0; nbk < NBK; ++nbk)
+                        mma16816<__half>(acc[nbk][mt], a0, a1, a2, a3, pb[nbk][j][0], pb[nbk][j][1]);
+                }
+            }
+            if (n + PF < N) ldsm_x4_t(st_v + chunk_off((n + PF) / NLD, (n + PF) % NLD), r[0], r[1], r[2], r[3]);
+        }
+    };
+
+    int4 merge = make_int4(0, 0, 0, 0);           // the unit that begins in this range and ends in a later one
+    if (w.g >= w.end) {
+        // nothing here: an empty partial, which a merge that spans this range passes over
+        for (int i = tc; i < p.GC; i += NCW * 32)
+            *reinterpret_cast<float2*>(p.ws_ml + ((size_t)2 * cta * p.GC + i) * 2) = make_float2(neg_inf, 0.0f);
+    }
+    while (w.g < w.end) {
+        const long long left = w.end - w.g;
+        const int n = (int)(left < (long long)(w.nt - w.ti) ? left : (long long)(w.nt - w.ti));
+        const bool begins = w.ti == 0, ends = w.ti + n == w.nt;
+        const int kv = w.ub / p.NCH, ch = w.ub % p.NCH;
+        const int gvalid = min(p.GC, p.G - ch * p.GC);
+        const int h0 = kv * p.G + ch * p.GC;
+        e0 = -1;
+        // ---- the unit's query rows as B fragments, each row scaled by a power of two into the range of a half
+#pragma unroll
+        for (int nbk = 0; nbk < NBK; ++nbk) {
+            const int head = nbk * HB + (SPLIT ? quad >> 1 : quad);
+            float4 x[KSTEPS];
+            float top = 0.0f;
+            bool odd = false;
+#pragma unroll
+            for (int kk = 0; kk < KSTEPS; ++kk) {
+                x[kk] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (head < gvalid) x[kk] = load4_any(p.q, ((size_t)w.b * p.Hq + h0 + head) * D + kk * 16 + qi * 4, p.out_dt);
+                top = fmaxf(top, fmaxf(fmaxf(fabsf(x[kk].x), fabsf(x[kk].y)), fmaxf(fabsf(x[kk].z), fabsf(x[kk].w))));
+                odd |= (x[kk].x != x[kk].x) | (x[kk].y != x[kk].y) | (x[kk].z != x[kk].z) | (x[kk].w != x[kk].w);
+            }
+            if (odd) top = INFINITY;
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            float fx, gx;
+            row_exponent(top, fx, gx);
+            const bool rest = SPLIT && (quad & 1);
+#pragma unroll
+            for (int kk = 0; kk < KSTEPS; ++kk) {
+                float e[4] = {x[kk].x * fx, x[kk].y * fx, x[kk].z * fx, x[kk].w * fx};
+                if (rest) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) e[c] -= __half2float(__float2half_rn(e[c]));
+                }
+                qb[nbk][kk][0] = pack2<__half>(e[0], e[1]);
+                qb[nbk][kk][1] = pack2<__half>(e[2], e[3]);
+            }
+#pragma unroll
+            for (int e = 0; e < HPT; ++e) {
+                kf[nbk][e] = __shfl_sync(0xffffffffu, gx, SPLIT ? 8 * qi : 4 * (2 * qi + e)) * p.scale * LOG2E;
+                m_run[nbk][e] = neg_inf;
+                l_run[nbk][e] = 0.0f;
+            }
+#pragma unroll
+            for (int mt = 0; mt < KSTEPS; ++mt) acc[nbk][mt][0] = acc[nbk][mt][1] = acc[nbk][mt][2] = acc[nbk][mt][3] = 0.0f;
+        }
+        // ---- this group's tiles of the segment
+        for (; own < i0 + n; own += Q8_NG) {
+            const bool ok = mbar_wait(bar_full + s * 8, ph, abort_flag, p.status, ST_WAIT_FULL_TIMEOUT);
+            const int rows_valid = w.len - (w.ti + (own - i0)) * TILE;      // >= 1
+            if (ok) {
+                if (rows_valid >= TILE) process(std::false_type{}, TILE);
+                else if (wr * (Q8_RB * 16) < rows_valid) process(std::true_type{}, rows_valid);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_empty + s * 8);
+            s += Q8_NG;
+            if (s >= Cfg::NS) { s -= Cfg::NS; ph ^= 1u; }
+        }
+        i0 += n;
+        // ---- fold the warps' states
+        const bool whole = begins && ends;
+        const float unit = e0 < 0 ? 1.0f : __uint_as_float((uint32_t)e0 << 23);      // 2^e0: sums of vs * v8 again
+        const size_t slot = (size_t)2 * cta + (begins ? 1 : 0);
+#pragma unroll
+        for (int nbk = 0; nbk < NBK; ++nbk) {
+            bar_consumers();                       // scratch is free again
+#pragma unroll
+            for (int e = 0; e < HPT; ++e) {
+                float l = l_run[nbk][e];
+                l += __shfl_xor_sync(0xffffffffu, l, 4);
+                l += __shfl_xor_sync(0xffffffffu, l, 8);
+                l += __shfl_xor_sync(0xffffffffu, l, 16);
+                const float m = m_run[nbk][e];
+                const int g = SPLIT ? qi : qi * 2 + e;
+                float* my = s_acc + ((size_t)warp * 8 + g) * Cfg::ACC_STRIDE + quad * 2;
+#pragma unroll
+                for (int mt = 0; mt < KSTEPS; ++mt) {
+                    float2 o;
+                    if constexpr (SPLIT) o = make_float2(acc[nbk][mt][0] + acc[nbk][mt][1], acc[nbk][mt][2] + acc[nbk][mt][3]);
+                    else o = make_float2(acc[nbk][mt][e], acc[nbk][mt][2 + e]);
+                    *reinterpret_cast<float2*>(my + mt * 16) = make_float2(o.x * unit, o.y * unit);
+                }
+                if (quad == 0) s_ml[warp * 8 + g] = make_float2(m, l);
+            }
+            bar_consumers();
+            for (int it = tc; it < HB * (D / 2); it += NCW * 32) {
+                const int row = it / (D / 2), d = (it % (D / 2)) * 2;
+                const int g = nbk * HB + row;
+                if (g >= gvalid) continue;
+                float mw[NCW];
+                float mg = neg_inf;
+#pragma unroll
+                for (int ww = 0; ww < NCW; ++ww) {
+                    mw[ww] = s_ml[ww * 8 + row].x;
+                    mg = fmaxf(mg, mw[ww]);
+                }
+                const float mg_safe = mg == neg_inf ? 0.0f : mg;
+                float a0 = 0.0f, a1 = 0.0f, lg = 0.0f;
+#pragma unroll
+                for (int ww = 0; ww < NCW; ++ww) {
+                    const float sc = ex2(mw[ww] - mg_safe);
+                    const float2 v = *reinterpret_cast<const float2*>(s_acc + ((size_t)ww * 8 + row) * Cfg::ACC_STRIDE + d);
+                    a0 += v.x * sc;
+                    a1 += v.y * sc;
+                    lg += s_ml[ww * 8 + row].y * sc;
+                }
+                if (whole) {
+                    const float inv = lg != 0.0f ? 1.0f / lg : 0.0f;
+                    store2_any(p.out, ((size_t)w.b * p.Hq + h0 + g) * D + d, p.out_dt, a0 * inv, a1 * inv);
+                } else if (FTK_SLOT_OK(p, slot, 0)) {
+                    const size_t pr = slot * p.GC + g;
+                    *reinterpret_cast<float2*>(p.ws_acc + pr * D + d) = make_float2(a0, a1);
+                    if (d == 0) *reinterpret_cast<float2*>(p.ws_ml + pr * 2) = make_float2(mg, lg);
+                }
+            }
+        }
+        if (begins && !ends) {
+            int last;
+            if (pl.ctot) {
+                last = cost_owner(pl, cost_of_unit(pl, w.b, w.ub, w.nt) + (long long)pl.ka * (w.nt - 1));
+            } else {
+                last = range_of(pl, w.g + w.nt - 1);              // w stands on the unit's first tile
+            }
+            merge = make_int4(w.b, w.ub, last - cta + 1, 0);
+        }
+        w.g += n - 1;
+        w.ti += n - 1;
+        walker_advance(p, w);
+    }
+    if (tc == 0) p.desc[cta] = merge;
+}
+
+// ---- generic kernel ---------------------------------------------------------------
+// Every other shape (head dims outside the list above or up to 512, blocks of other than a power of two >= 16 rows,
+// unaligned operands, more sequences than the schedule's table holds): CUDA cores, float32 throughout. One CTA per (unit of
+// up to 4 heads, range): a unit's rows are cut into nsplit equal ranges, a warp takes every eighth group of 4 rows, a lane
+// every 32nd word of 4 codes. Bound by instruction issue (the 5-step reductions of the scores), not by bandwidth.
+constexpr int Q8G_HEADS = 4;
+template <typename KV, int LC>
+__global__ void __launch_bounds__(256)
+decode_q8_generic_kernel(const Q8Params p) {
+    __shared__ float s_acc[8][LC * 128];
+    __shared__ float2 s_ml[8][Q8G_HEADS];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int upb = p.Hkv * p.NCH;
+    const long long unit = blockIdx.x / (unsigned)p.nsplit;
+    const int part = (int)(blockIdx.x - unit * p.nsplit);
+    const int b = (int)(unit / upb), ub = (int)(unit - (long long)b * upb);
+    const int kv = ub / p.NCH, ch = ub % p.NCH;
+    const int gvalid = min(Q8G_HEADS, p.G - ch * Q8G_HEADS);
+    const int h0 = kv * p.G + ch * Q8G_HEADS;
+    const int len = seq_len(p, b);
+    const int per = (len + p.nsplit - 1) / p.nsplit;
+    const int begin = min(len, part * per), end = min(len, begin + per);
+    const int words = p.D >> 2;
+    float4 q[Q8G_HEADS][LC], acc[Q8G_HEADS][LC];
+    float m[Q8G_HEADS], l[Q8G_HEADS];
+#pragma unroll
+    for (int g = 0; g < Q8G_HEADS; ++g) {
+        m[g] = -INFINITY;
+        l[g] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < LC; ++c) {
+            q[g][c] = acc[g][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (g < gvalid && lane + 32 * c < words)
+                q[g][c] = load4_any(p.q, ((size_t)b * p.Hq + h0 + g) * p.D + (size_t)(lane + 32 * c) * 4, p.out_dt);
+        }
+    }
+    const float to2 = p.scale * LOG2E;
+    constexpr int R = 4;
+    for (int t0 = begin + warp * R; t0 < end; t0 += 8 * R) {
+        uint32_t kw[R][LC], vw[R][LC];
+        float2 sc[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int t = min(t0 + r, end - 1);
+            int blk = __ldg(p.table + (size_t)b * p.tbl_width + t / p.page);
+            if (!(blk >= 0 && blk < p.blocks)) blk = 0;
+            sc[r] = __ldg(p.scales + (size_t)blk * p.Hkv + kv);
+            const size_t row = ((size_t)blk * p.Hkv + kv) * p.page + t % p.page;
+#pragma unroll
+            for (int c = 0; c < LC; ++c) {
+                kw[r][c] = vw[r][c] = 0;
+                if (lane + 32 * c < words) {
+                    kw[r][c] = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(p.k) + row * p.D) + lane + 32 * c);
+                    vw[r][c] = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(p.v) + row * p.D) + lane + 32 * c);
+                }
+            }
+        }
+        float s[R][Q8G_HEADS];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+            for (int g = 0; g < Q8G_HEADS; ++g) s[r][g] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < LC; ++c) {
+                const float4 k = Codes<KV>::floats(kw[r][c]);
+#pragma unroll
+                for (int g = 0; g < Q8G_HEADS; ++g)
+                    s[r][g] = fmaf(q[g][c].w, k.w, fmaf(q[g][c].z, k.z, fmaf(q[g][c].y, k.y, fmaf(q[g][c].x, k.x, s[r][g]))));
+            }
+#pragma unroll
+            for (int g = 0; g < Q8G_HEADS; ++g) {
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) s[r][g] += __shfl_xor_sync(0xffffffffu, s[r][g], o);
+                s[r][g] = t0 + r < end ? s[r][g] * (sc[r].x * to2) : -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < Q8G_HEADS; ++g) {
+            float mx = m[g];
+#pragma unroll
+            for (int r = 0; r < R; ++r) mx = fmaxf(mx, s[r][g]);
+            const float safe = mx == -INFINITY ? 0.0f : mx;
+            const float alpha = ex2(m[g] - safe);
+            m[g] = mx;
+            l[g] *= alpha;
+#pragma unroll
+            for (int c = 0; c < LC; ++c) { acc[g][c].x *= alpha; acc[g][c].y *= alpha; acc[g][c].z *= alpha; acc[g][c].w *= alpha; }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float w8 = ex2(s[r][g] - safe);
+                l[g] += w8;
+                s[r][g] = t0 + r < end ? w8 * sc[r].y : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (t0 + r >= end) break;
+#pragma unroll
+            for (int c = 0; c < LC; ++c) {
+                const float4 v = Codes<KV>::floats(vw[r][c]);
+#pragma unroll
+                for (int g = 0; g < Q8G_HEADS; ++g) {
+                    acc[g][c].x = fmaf(s[r][g], v.x, acc[g][c].x);
+                    acc[g][c].y = fmaf(s[r][g], v.y, acc[g][c].y);
+                    acc[g][c].z = fmaf(s[r][g], v.z, acc[g][c].z);
+                    acc[g][c].w = fmaf(s[r][g], v.w, acc[g][c].w);
+                }
+            }
+        }
+    }
+    if (lane == 0)
+#pragma unroll
+        for (int g = 0; g < Q8G_HEADS; ++g) s_ml[warp][g] = make_float2(m[g], l[g]);
+#pragma unroll
+    for (int g = 0; g < Q8G_HEADS; ++g) {
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < LC; ++c) *reinterpret_cast<float4*>(&s_acc[warp][(lane + 32 * c) * 4]) = acc[g][c];
+        __syncthreads();
+        if (g >= gvalid) continue;
+        for (int d = threadIdx.x * 2; d < p.D; d += 512) {
+            float mg = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) mg = fmaxf(mg, s_ml[w][g].x);
+            const float safe = mg == -INFINITY ? 0.0f : mg;
+            float a0 = 0.0f, a1 = 0.0f, lg = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) {
+                const float f = ex2(s_ml[w][g].x - safe);
+                a0 += s_acc[w][d] * f;
+                a1 += s_acc[w][d + 1] * f;
+                lg += s_ml[w][g].y * f;
+            }
+            if (p.nsplit == 1) {
+                const float inv = lg != 0.0f ? 1.0f / lg : 0.0f;
+                store2_any(p.out, ((size_t)b * p.Hq + h0 + g) * p.D + d, p.out_dt, a0 * inv, a1 * inv);
+            } else {
+                const size_t pr = (size_t)blockIdx.x * Q8G_HEADS + g;
+                *reinterpret_cast<float2*>(p.ws_acc + pr * p.D + d) = make_float2(a0, a1);
+                if (d == 0) *reinterpret_cast<float2*>(p.ws_ml + pr * 2) = make_float2(mg, lg);
+            }
+        }
+    }
+}
+
+// ---- merge -------------------------------------------------------------------------
+// Folds the partials of the units that were cut. TC: block c looks at the unit that begins in range c of the tensor-core
+// kernel and ends in a later one, if any: its first partial is slot 2 c + 1, the next ones the even slots behind.
+// Otherwise block u folds the nsplit slots of unit u of the generic kernel. Weights 2^(m_j - max m) worked out once per
+// (partial, head) in shared memory; the sums run over the partials in order, four float4 loads in flight per thread.
+constexpr int Q8M_THREADS = 128;
+constexpr int Q8M_ROUND = 1024;                     // (partial, head) weights per round
+template <bool TC>
+__global__ void __launch_bounds__(Q8M_THREADS) q8_merge_kernel(const Q8Params p) {
+    __shared__ float s_w[Q8M_ROUND];
+    __shared__ float s_top[16], s_l[16];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int c = (int)blockIdx.x, tid = threadIdx.x;
+    const int upb = p.Hkv * p.NCH;
+    int b, ub, parts;
+    if (TC) {
+        const int4 d = __ldcg(p.desc + c);
+        if (d.z < 2) return;
+        b = d.x; ub = d.y; parts = d.z;
+    } else {
+        b = c / upb; ub = c - b * upb; parts = p.nsplit;
+    }
+    auto slot = [&](int j) -> size_t { return TC ? (j ? (size_t)2 * (c + j) : (size_t)2 * c + 1) : (size_t)c * parts + j; };
+    const int kv = ub / p.NCH, ch = ub % p.NCH;
+    const int gv = min(p.GC, p.G - ch * p.GC);
+    const int h0 = kv * p.G + ch * p.GC;
+    // the largest exponent of each head, a warp per head
+    const int warp = tid >> 5, lane = tid & 31;
+    for (int g = warp; g < gv; g += Q8M_THREADS / 32) {
+        float top = -INFINITY;
+        for (int j = lane; j < parts; j += 32) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml + (slot(j) * p.GC + g) * 2));
+            if (ml.y != 0.0f) top = fmaxf(top, ml.x);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (top == -INFINITY) top = 0.0f;
+        float sum = 0.0f;
+        for (int j = lane; j < parts; j += 32) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml + (slot(j) * p.GC + g) * 2));
+            if (ml.y != 0.0f) sum += ml.y * ex2(ml.x - top);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) { s_top[g] = top; s_l[g] = sum; }
+    }
+    const int quads = p.D >> 2, items = gv * quads;
+    const int round = Q8M_ROUND / gv;
+    for (int i0 = 0; i0 < items; i0 += Q8M_THREADS) {
+        const int it = i0 + tid;
+        const int g = it < items ? it / quads : 0, d = it < items ? (it - g * quads) * 4 : 0;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int j0 = 0; j0 < parts; j0 += round) {
+            const int n = min(round, parts - j0);
+            if (i0 == 0 || parts > round) {
+                __syncthreads();
+                for (int k = tid; k < n * gv; k += Q8M_THREADS) {
+                    const int gg = k % gv;
+                    const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml + (slot(j0 + k / gv) * p.GC + gg) * 2));
+                    s_w[k] = ml.y != 0.0f ? ex2(ml.x - s_top[gg]) : -1.0f;         // -1: an empty partial, its sums unwritten
+                }
+                __syncthreads();
+            }
+            if (it < items) {
+#pragma unroll 4
+                for (int j = 0; j < n; ++j) {
+                    const float f = s_w[j * gv + g];
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (f >= 0.0f || f != f) v = __ldcg(reinterpret_cast<const float4*>(p.ws_acc + (slot(j0 + j) * p.GC + g) * p.D + d));
+                    a.x = fmaf(v.x, f, a.x); a.y = fmaf(v.y, f, a.y); a.z = fmaf(v.z, f, a.z); a.w = fmaf(v.w, f, a.w);
+                }
+            }
+        }
+        if (it < items) {
+            const float l = s_l[g];
+            const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+            store4_any(p.out, ((size_t)b * p.Hq + h0 + g) * p.D + d, p.out_dt, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
+        }
+    }
+}
+
+}  // namespace ftk

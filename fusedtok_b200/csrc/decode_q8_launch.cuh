@@ -1,0 +1,36 @@
+// Kernel instantiations of the 8-bit decode for one code type and one group of head dims, and their launch: included by
+// decode_q8_<codes>_<dims>.cu so that they compile side by side.
+#pragma once
+
+#include "decode_q8.cuh"
+
+namespace ftk {
+
+template <typename KV, int D, int NBK, bool SPLIT>
+cudaError_t q8_launch_one(const CUtensorMap& mk, const CUtensorMap& mv, const Q8Params& p, cudaStream_t cs) {
+    // a function attribute, not a stream operation: cheap, and legal while the stream is captured
+    cudaError_t e = cudaFuncSetAttribute(decode_q8_kernel<KV, D, NBK, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         Q8Cfg<D>::SMEM_BYTES);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.ncta);
+    cfg.blockDim = dim3(TC_THREADS);
+    cfg.dynamicSmemBytes = Q8Cfg<D>::SMEM_BYTES;
+    cfg.stream = cs;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, decode_q8_kernel<KV, D, NBK, SPLIT>, mk, mv, p);
+}
+
+template <typename KV, int D>
+cudaError_t q8_launch_dim(const CUtensorMap& mk, const CUtensorMap& mv, const Q8Params& p, int nbk, bool split, cudaStream_t cs) {
+    if constexpr (D <= 128) {
+        if (nbk == 2) return split ? q8_launch_one<KV, D, 2, true>(mk, mv, p, cs) : q8_launch_one<KV, D, 2, false>(mk, mv, p, cs);
+    }
+    return split ? q8_launch_one<KV, D, 1, true>(mk, mv, p, cs) : q8_launch_one<KV, D, 1, false>(mk, mv, p, cs);
+}
+
+}  // namespace ftk

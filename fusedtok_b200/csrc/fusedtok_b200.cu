@@ -20,6 +20,7 @@
 #include <vector>
 
 #include "common.cuh"
+#include "host.h"
 #include "decode_simt.cuh"
 #include "decode_tc.cuh"
 #include "decode_ring.cuh"
@@ -79,10 +80,7 @@ struct DeviceState {
 DeviceState g_dev[kMaxDevices];
 std::mutex g_mutex;
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
-                                  CUtensorMapFloatOOBfill);
+using host::EncodeTiledFn;
 EncodeTiledFn g_encode = nullptr;
 
 int get_encode_fn() {
@@ -954,6 +952,29 @@ int rope_append_common(int dt, int neox, const void* q, void* q_out, const void*
     return check_launch("rope + kv append kernel launch");
 }
 
+}  // namespace
+
+// the parts of the above that the other translation units use (host.h)
+namespace ftk {
+namespace host {
+int fail(int code, const std::string& msg) { return ::fail(code, msg); }
+int launched(const char* what) { return check_launch(what); }
+int current_sm_count(int* count) {
+    DeviceState* dev = nullptr;
+    const int rc = device_state(&dev);
+    if (rc == FUSEDTOK_OK) *count = dev->sm_count;
+    return rc;
+}
+int encoder(EncodeTiledFn* fn) {
+    const int rc = get_encode_fn();
+    if (rc == FUSEDTOK_OK) *fn = g_encode;
+    return rc;
+}
+}  // namespace host
+}  // namespace ftk
+
+namespace {
+
 // RAII device buffer for the staged paths (reference: DevBuf, src/bindings.cpp:47-66)
 struct DevBuf {
     void* p = nullptr;
@@ -1551,6 +1572,10 @@ int fusedtok_attention_device_status(int* status) {
             if (*status == 0) *status = word;
         }
     }
+    word = 0;
+    const int rc8 = ftk::host::q8_status(&word);
+    if (rc8) return rc8;
+    if (*status == 0) *status = word;
     return FUSEDTOK_OK;
 }
 

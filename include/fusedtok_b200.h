@@ -287,13 +287,90 @@ int fusedtok_attention_decode_launch_noalloc(int dtype, const void* q, const voi
                                              const int* lens, void* out, int batch, int q_heads,
                                              int kv_heads, int cache_rows, int dim, uintptr_t stream);
 
+/* ---- paged cache held in 8 bits (no counterpart in the reference) ------------
+ * Pools k, v [Nb, Hkv, P, D] of one-byte codes - store 0: int8 (-127..127),
+ * store 1: e4m3 - and kv_scales [Nb, Hkv, 2] float32: row (block, head, offset)
+ * of K stands for code * kv_scales[block][head][0], of V for
+ * code * kv_scales[block][head][1]. dtype (of q / out / k_new / v_new): 0
+ * float32, 1 bfloat16, 2 float16. All pointers are device memory, all calls
+ * asynchronous on `stream` and capturable, also as the first call on a device;
+ * none allocates, and none keeps anything between calls, so calls on different
+ * streams and captured graphs may overlap as long as their operands do not.
+ *
+ * attention_decode_paged_q8: fusedtok_attention_decode_paged_launch over such a
+ * cache (same shapes, head mapping, scale and zero rows; any GQA group; a block
+ * table entry outside [0, num_blocks) is read as block 0). Accumulation in float32.
+ * `workspace`: 16-byte aligned device memory of at least
+ * fusedtok_attention_decode_paged_q8_workspace(...) bytes that the call may
+ * overwrite and no other work may touch until it is done (its contents before
+ * do not matter; a negative return value is minus the status code of a shape
+ * that the launcher would refuse). q and out aligned to 4 elements, pools to 4
+ * bytes (16 for the fast kernel), kv_scales to 8.
+ *
+ * kv_append_paged_q8: token i's rows k_new[i], v_new[i] ([N, Hkv, D]) are rounded
+ * into the cache at slots[i] = block * P + offset; a slot outside
+ * [0, Nb * P) passes the token over. Tokens with consecutive slots inside one
+ * block form a run; all tokens of a call that go to one block have to form one
+ * run. Per kv head, and for K and V each, with o the run's first offset, M =
+ * 127 (int8) or 448 (e4m3) and round() to the nearest code of the exact
+ * quotient, ties to even:
+ *     old = o > 0 ? scale : 0,  new = max(old, max|x| / M);
+ *     rows before o: code = round(code * old / new); the run's: round(x / new).
+ * Rows behind the run keep their codes (they stand for nothing until they are
+ * appended). new == 0 gives codes 0; a NaN or infinity among the run's values
+ * makes the scale NaN, and the block reads as NaN until it is begun again at
+ * offset 0. D % 4 == 0, D <= 512, Nb * P < 2^31. */
+long long fusedtok_attention_decode_paged_q8_workspace(int dtype, int batch, int q_heads, int kv_heads, int page,
+                                                       int tbl_width, int dim);
+int fusedtok_attention_decode_paged_q8_launch(int dtype, int store, const void* q, const void* k_pool,
+                                              const void* v_pool, const float* kv_scales, const int* table,
+                                              const int* lens, void* out, void* workspace, long long workspace_bytes,
+                                              int batch, int q_heads, int kv_heads, int page, int tbl_width,
+                                              long long num_blocks, int dim, uintptr_t stream);
+int fusedtok_kv_append_paged_q8_launch(int dtype, int store, const void* k_new, const void* v_new, const int* slots,
+                                       void* k_pool, void* v_pool, float* kv_scales, int tokens, int kv_heads, int dim,
+                                       int page, long long num_blocks, uintptr_t stream);
+
+/* ---- block tables and slot maps from request lengths, on the GPU (no counterpart
+ * in the reference, which takes the table as given) ------------------------------
+ * The free blocks are a stack: free_blocks[0 .. *free_count). Sequence b holds
+ * lens[b] tokens in blocks table[b][0 .. ceil(lens[b] / P)).
+ *
+ * extend: b is to grow by new_lens[b] tokens. The tokens of the batch are numbered
+ * in order, starts[b] being the first of b's (starts[batch]: one past the last).
+ * With fits = (lens[b] + new_lens[b] <= tbl_width * P and starts[b + 1] <=
+ * max_tokens), ask = fits ? blocks missing : 0 and upto = its inclusive sum over
+ * the batch, b is granted if fits and (ask == 0 or upto <= *free_count): the
+ * blocks go out in batch order, and the first sequence that cannot be served
+ * ends it for every later one that needs a block. The k-th block asked for is
+ * free_blocks[*free_count - 1 - k]; granted ones are written into the table.
+ * slots[t] = block * P + offset for the tokens of granted sequences, -1 for the
+ * others and behind the last token; lens_out[b] = lens[b] + new_lens[b] if
+ * granted, else lens[b]; *free_count_out = what is left. free_blocks is only read.
+ *
+ * trim: b is cut back to min(lens[b], keep_lens[b]) tokens (0: finished). The
+ * blocks no longer needed are pushed in batch order: free_blocks[*free_count],
+ * ...; lens_out and *free_count_out are the new lengths and count. The table is
+ * only read; its entries behind the new lengths stand for nothing.
+ *
+ * Negative lengths count as 0. At most 8192 sequences. lens_out and
+ * free_count_out must not overlap the inputs. Asynchronous, capturable, no
+ * workspace. */
+int fusedtok_block_table_extend_launch(int* table, const int* lens, const int* new_lens, const int* free_blocks,
+                                       const int* free_count, int* slots, int* starts, int* lens_out,
+                                       int* free_count_out, int batch, int tbl_width, int page, int free_capacity,
+                                       int max_tokens, uintptr_t stream);
+int fusedtok_block_table_trim_launch(const int* table, const int* lens, const int* keep_lens, int* free_blocks,
+                                     const int* free_count, int* lens_out, int* free_count_out, int batch,
+                                     int tbl_width, int page, int free_capacity, uintptr_t stream);
+
 /* ---- diagnostics -----------------------------------------------------------
  * Every device-side wait in the kernels is bounded; a wait that expires stores
  * a non-zero code in a per-device status word and the kernel still completes.
  * This call synchronises the current device, returns the word through
  * `status` (0 = ok) and clears it. It covers both the workspace the allocating
  * launchers own and the static scratch of the allocation-free launcher (the
- * first non-zero of the two is returned); after a non-zero word the arrival
+ * first non-zero of the two is returned), and the 8-bit decode's own word; after a non-zero word the arrival
  * counters of that path are cleared too, so the next launch starts clean. */
 int fusedtok_attention_device_status(int* status);
 

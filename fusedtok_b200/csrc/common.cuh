@@ -824,7 +824,7 @@ __device__ __forceinline__ unsigned long long timeline_ns() {
     return t;
 }
 #ifdef FTK_TIMELINE
-__device__ unsigned long long g_timeline[1024][24];
+static __device__ unsigned long long g_timeline[1024][24];
 #define FTK_STAMP(cond, slot) do { if (cond) g_timeline[blockIdx.x][slot] = timeline_ns(); } while (0)
 #define FTK_ADD(cond, slot, v) do { if (cond) g_timeline[blockIdx.x][slot] += (v); } while (0)
 #define FTK_NOW() timeline_ns()

@@ -6,9 +6,16 @@
 // registers, on its way from shared memory to the tensor cores. Both code types are exact in half precision, and
 // the scales never touch the codes: ks multiplies the finished score, vs is folded into the softmax weight.
 //
-// Structure (see decode_tc.cuh for the parts both share): one persistent CTA per SM, 1 producer warp that streams
-// 64-row tiles with TMA into a ring in shared memory, 8 consumer warps; all tiles of all units cut at equal cost
-// into one range per CTA, worked out on the device from lens.
+// Structure (see decode_tc.cuh for the parts both share): one persistent CTA per SM; all tiles of all units cut at equal
+// cost into one range per CTA, worked out on the device from lens. Three kinds of warps, every one walking the range for
+// itself:
+//  * 4 producer warps stream 64-row tiles with TMA into a ring in shared memory, one for each group of consumer warps;
+//  * 8 consumer warps, in 4 groups that take tiles in turn, keep an online softmax over their rows in registers. Nothing
+//    makes them meet: at the end of a segment (the range's part of a unit) a warp leaves its state (m, l, O) in a buffer
+//    and goes on;
+//  * 4 helper warps prepare the query fragments of the next segment and fold the 8 states of the last one. With both done
+//    by the consumers, and barriers between them, every segment cost a CTA about 4 us (12 tiles' worth), and 64 ragged
+//    sequences took 130 us instead of 95.
 //  * Stage layout: a block's (page x D) bytes are contiguous in the pool, so the pool is described to TMA as 128-byte
 //    lines with the 128-byte swizzle, whatever D is; row r, 16-byte chunk c of a tile sits at line-linear address
 //    r * D + 16 c, swizzled. One copy per block and tile for K, one for V; the two scales of the block follow with an
@@ -42,6 +49,9 @@ namespace ftk {
 constexpr int Q8_WPT = 2;                       // consumer warps per tile
 constexpr int Q8_NG = NCW / Q8_WPT;             // groups of warps, taking tiles in turn
 constexpr int Q8_RB = 4 / Q8_WPT;               // 16-row blocks of a tile per warp
+constexpr int Q8_HELPERS = 4;                   // helper warps
+constexpr int Q8_THREADS = (NCW + Q8_HELPERS + Q8_NG) * 32;   // ... and a producer warp per group
+static_assert(Q8_THREADS == 512, "the register split below counts 16 warps");
 constexpr int Q8_MAX_SPLIT = 32;                // generic kernel: most ranges a unit is cut into
 
 struct Q8Params : DecodeParams {
@@ -115,7 +125,7 @@ template <> struct Codes<__nv_fp8_e4m3> {
     }
 };
 
-template <int D> struct Q8Cfg {
+template <int D, int NBK, bool SPLIT> struct Q8Cfg {
     static_assert(D % 16 == 0 && D >= 64 && D <= 256, "head dim: a multiple of 16 from 64 to 256");
     static constexpr int KV_BYTES = TILE * D;          // a multiple of 1024: the swizzle phase of every stage is the same
     static constexpr int STAGE_BYTES = 2 * KV_BYTES;
@@ -123,13 +133,21 @@ template <int D> struct Q8Cfg {
     // always consumed by the same group, which then sees every phase of its barrier in order
     static constexpr int NS = (131072 / STAGE_BYTES) / Q8_NG * Q8_NG;
     static_assert(NS >= Q8_NG, "ring shorter than the groups");
+    static constexpr int HEADS = NBK * (SPLIT ? 4 : 8);
     static constexpr int ACC_STRIDE = D + 4;
-    static constexpr int SCRATCH_BYTES = NCW * 8 * ACC_STRIDE * 4;
-    static constexpr int OFF_SCRATCH = NS * STAGE_BYTES;
-    static constexpr int OFF_ML = OFF_SCRATCH + SCRATCH_BYTES;       // [NCW][8] (m, l)
-    static constexpr int OFF_SCALE = OFF_ML + NCW * 8 * 8;           // [NS][4] (K, V) scales of the stage's blocks
-    static constexpr int OFF_BAR = OFF_SCALE + NS * 4 * 8;           // full[NS], empty[NS]
-    static constexpr int OFF_SCHED = OFF_BAR + 2 * NS * 8;
+    static constexpr int STATE_BYTES = NCW * HEADS * ACC_STRIDE * 4;             // the warps' O of one segment
+    static constexpr int NF = STATE_BYTES <= 34816 ? 2 : 1;                      // segments whose states may wait to be folded
+    static constexpr int Q_BYTES = NBK * (D / 16) * 32 * 8;                      // query fragments of a segment
+    // The CTA is launched with 128 registers per thread; the 2 consumer warpgroups take more, the 2 others give up as many.
+    static constexpr int REGS_CONSUMER = NBK * D <= 128 ? 152 : 168, REGS_OTHER = 256 - REGS_CONSUMER;
+    static constexpr int OFF_STATE = NS * STAGE_BYTES;
+    static constexpr int OFF_ML = OFF_STATE + NF * STATE_BYTES;                  // [NF][NCW][HEADS] (m, l)
+    static constexpr int OFF_Q = OFF_ML + NF * NCW * HEADS * 8;                  // [2] fragments
+    static constexpr int OFF_KF = OFF_Q + 2 * Q_BYTES;                           // [2][16] score factors
+    static constexpr int OFF_W = OFF_KF + 2 * 16 * 4;                            // [HEADS][NCW] weights of the fold, [HEADS] l
+    static constexpr int OFF_SCALE = OFF_W + 16 * (NCW + 1) * 4;                 // [NS][4] (K, V) scales of the stage's blocks
+    static constexpr int OFF_BAR = OFF_SCALE + NS * 4 * 8;                       // full[NS], empty[NS], q full / empty [2], state full / empty [2]
+    static constexpr int OFF_SCHED = OFF_BAR + (2 * NS + 8) * 8;
     static constexpr int OFF_ABORT = OFF_SCHED + (int)sizeof(SchedShared);
     static constexpr int OFF_PREFIX = (OFF_ABORT + 16 + 15) & ~15;
     static constexpr int OFF_ZPRE = OFF_PREFIX + (SCHED_MAX_B + 1) * 4;
@@ -163,15 +181,17 @@ __device__ __forceinline__ void row_exponent(float x, float& f, float& g) {
 // ---- the kernel ----------------------------------------------------------------
 // KV: code type. NBK: 8-column blocks of the MMA. SPLIT: two columns per query head (see above).
 template <typename KV, int D, int NBK, bool SPLIT>
-__global__ void __launch_bounds__(TC_THREADS, 1)
+__global__ void __launch_bounds__(Q8_THREADS, 1)
 decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Q8Params p) {
-    using Cfg = Q8Cfg<D>;
+    using Cfg = Q8Cfg<D, NBK, SPLIT>;
     extern __shared__ __align__(1024) uint8_t smem[];
     SchedShared* sh = reinterpret_cast<SchedShared*>(smem + Cfg::OFF_SCHED);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Cfg::OFF_ABORT);
     const uint32_t smem_base = smem_u32(smem);
     const uint32_t bar_full = smem_base + Cfg::OFF_BAR;
     const uint32_t bar_empty = bar_full + Cfg::NS * 8;
+    const uint32_t bar_q_full = bar_empty + Cfg::NS * 8, bar_q_empty = bar_q_full + 16;
+    const uint32_t bar_state_full = bar_q_empty + 16, bar_state_empty = bar_state_full + 16;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int cta = (int)blockIdx.x;
 
@@ -184,6 +204,12 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         for (int s = 0; s < Cfg::NS; ++s) {
             mbar_init(bar_full + s * 8, 33);           // the announced bytes, and each producer lane's scales
             mbar_init(bar_empty + s * 8, Q8_WPT);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(bar_q_full + s * 8, Q8_HELPERS);
+            mbar_init(bar_q_empty + s * 8, NCW);
+            mbar_init(bar_state_full + s * 8, NCW);
+            mbar_init(bar_state_empty + s * 8, Q8_HELPERS);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_k) : "memory");
@@ -222,34 +248,48 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         else if (!range_empty(pl, cta)) w = walker_locate(p, prefix, range_start(pl, cta), range_start(pl, cta + 1));
     }
 
-    if (warp == NCW) {
-        // ===================== producer warp =====================
+    constexpr int KSTEPS = D / 16;
+    constexpr int HB = SPLIT ? 4 : 8;              // query heads per column block
+    constexpr int HEADS = Cfg::HEADS;
+
+    if (warp >= NCW + Q8_HELPERS) {
+        // ===================== producer warps =====================
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_OTHER));
+        // One per group of consumer warps: it issues that group's tiles (every Q8_NG-th of the range). A single one would
+        // have to issue a 16 KB tile of 2 KB blocks every 350 ns, and falls behind (measured: 94 us instead of 47).
+        const int cg = warp - NCW - Q8_HELPERS;
         const uint64_t pol = policy_evict_first();
-        const int* tbl = nullptr;
-        int issued = 0, s = 0;
+        const int page_shift = __ffs(p.page) - 1;
+        const int per_tile = 1 << (6 - p.box_shift);                        // blocks (or parts of one) a tile has
+        // Table entries, one per lane: lane (k, j) holds block j of this warp's k-th next tile, as far as the unit goes,
+        // and another set the entries of the tiles behind those, on their way
+        const int lane_row = (lane >> (6 - p.box_shift)) * (Q8_NG * TILE) + ((lane & (per_tile - 1)) << p.box_shift);
+        const int reach = 32 >> (6 - p.box_shift);                          // tiles a set covers
+        int at = reach, tbl_val = 0, tbl_next = 0, unit_b = -1, unit_ub = -1;
+        int issued = 0, s = cg;
         uint32_t ph = 0;
-        // 32 consecutive table entries of the current sequence, one per lane, and the 32 behind them, already on their way
-        int tbl_b = -1, tbl_base = 0, tbl_val = 0, tbl_next = 0;
         bool gave_up = false;
+        for (int i = 0; i < cg && w.g < w.end; ++i) walker_advance(p, w);
         while (w.g < w.end) {
             const int kv = w.ub / p.NCH;
             const int t0 = w.ti * TILE;
-            const int pg0 = p.page <= TILE ? t0 >> p.box_shift : t0 / p.page;
-            const int npg = p.page <= TILE ? (min(TILE, w.len - t0) + p.page - 1) >> p.box_shift : 1;
-            if (tbl_b != w.b || pg0 < tbl_base || pg0 + npg > tbl_base + 32) {
-                tbl = p.table + (size_t)w.b * p.tbl_width;
-                if (tbl_b == w.b && pg0 == tbl_base + 32) {
-                    tbl_val = tbl_next;
-                } else {
-                    tbl_val = pg0 + lane < p.tbl_width ? __ldg(tbl + pg0 + lane) : 0;
-                }
-                tbl_base = pg0;
-                tbl_b = w.b;
-                tbl_next = pg0 + 32 + lane < p.tbl_width ? __ldg(tbl + pg0 + 32 + lane) : 0;
+            auto entry = [&](int row) { return row < w.len ? __ldg(p.table + (size_t)w.b * p.tbl_width + (row >> page_shift)) : 0; };
+            if (w.b != unit_b || w.ub != unit_ub) {
+                unit_b = w.b;
+                unit_ub = w.ub;
+                at = 0;
+                tbl_val = entry(t0 + lane_row);
+                tbl_next = entry(t0 + reach * (Q8_NG * TILE) + lane_row);
+            } else if (at == reach) {
+                at = 0;
+                tbl_val = tbl_next;
+                tbl_next = entry(t0 + reach * (Q8_NG * TILE) + lane_row);
             }
-            int blk = __shfl_sync(0xffffffffu, tbl_val, (pg0 - tbl_base + lane) & 31);
+            const int npg = p.page <= TILE ? (min(TILE, w.len - t0) + p.page - 1) >> p.box_shift : 1;
+            int blk = __shfl_sync(0xffffffffu, tbl_val, (at * per_tile + lane) & 31);
+            ++at;
             if (lane < npg && !(blk >= 0 && blk < p.blocks)) blk = 0;      // (device table values are trusted: address only)
-            const long long unit_row = ((long long)blk * p.Hkv + kv) * p.page + (p.page <= TILE ? 0 : t0 - pg0 * p.page);
+            const long long unit_row = ((long long)blk * p.Hkv + kv) * p.page + (p.page <= TILE ? 0 : t0 & (p.page - 1));
             const int line = (int)(unit_row * D >> 7);
             const uint32_t bytes = (uint32_t)(npg << p.box_shift) * (uint32_t)(2 * D);
             if (!mbar_wait(bar_empty + s * 8, ph ^ 1u, abort_flag, p.status, ST_WAIT_EMPTY_TIMEOUT)) {
@@ -267,16 +307,24 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
             }
             cp_async_arrive(fb);
             ++issued;
-            walker_advance(p, w);
-            if (++s == Cfg::NS) { s = 0; ph ^= 1u; }
+            if (w.ti + Q8_NG < w.nt) {
+                w.g += Q8_NG;
+                w.ti += Q8_NG;
+            } else {
+                for (int i = 0; i < Q8_NG && w.g < w.end; ++i) walker_advance(p, w);
+            }
+            s += Q8_NG;
+            if (s >= Cfg::NS) { s -= Cfg::NS; ph ^= 1u; }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         if (gave_up || *abort_flag) {
-            // do not leave the CTA while its own copies may still be landing: wait (bounded) for every stage issued
-            const int first = issued > Cfg::NS ? issued - Cfg::NS : 0;
+            // do not leave the CTA while its own copies may still be landing: wait (bounded) for the last phase of every
+            // stage this warp issued
+            constexpr int OWN = Cfg::NS / Q8_NG;
+            const int first = issued > OWN ? issued - OWN : 0;
             for (int i = first; i < issued; ++i) {
                 const unsigned long long b0 = global_ns();
-                while (!mbar_try_wait(bar_full + (i % Cfg::NS) * 8, (uint32_t)((i / Cfg::NS) & 1))) {
+                while (!mbar_try_wait(bar_full + (cg + (i % OWN) * Q8_NG) * 8, (uint32_t)((i / OWN) & 1))) {
                     if (global_ns() - b0 > WAIT_LIMIT_NS) {
                         atomicCAS(p.status, ST_OK, ST_DRAIN_TIMEOUT);
                         break;
@@ -287,18 +335,152 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         return;
     }
 
+    if (warp >= NCW) {
+        // ===================== helper warps =====================
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_OTHER));
+        const int hw = warp - NCW, tid = threadIdx.x - NCW * 32;
+        float* s_w = reinterpret_cast<float*>(smem + Cfg::OFF_W);
+        auto helpers = [] { asm volatile("bar.sync 2, %0;" ::"n"(Q8_HELPERS * 32) : "memory"); };
+        // The query rows of a unit as B fragments, each row scaled by a power of two into the range of a half. A warp
+        // takes every fourth head; a lane the 4 elements that make a fragment register pair.
+        auto prepare_q = [&](int k, const Walker& u) {
+            const int buf = k & 1;
+            mbar_wait(bar_q_empty + buf * 8, (uint32_t)((k >> 1) & 1) ^ 1u, abort_flag, p.status, ST_WAIT_RANGE_TIMEOUT);
+            const int kv = u.ub / p.NCH, ch = u.ub % p.NCH;
+            const int gvalid = min(p.GC, p.G - ch * p.GC);
+            const size_t row0 = ((size_t)u.b * p.Hq + kv * p.G + ch * p.GC) * D;
+            uint2* frag = reinterpret_cast<uint2*>(smem + Cfg::OFF_Q + buf * Cfg::Q_BYTES);
+            float* kf = reinterpret_cast<float*>(smem + Cfg::OFF_KF) + buf * 16;
+            constexpr int PER = (HEADS + Q8_HELPERS - 1) / Q8_HELPERS, LR = (D / 4 + 31) / 32;
+            float4 x[PER][LR];
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+#pragma unroll
+                for (int r = 0; r < LR; ++r) {
+                    const int g = hw + i * Q8_HELPERS, c = lane + 32 * r;
+                    x[i][r] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (g < gvalid && c < D / 4) x[i][r] = load4_any(p.q, row0 + (size_t)g * D + c * 4, p.out_dt);
+                }
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int g = hw + i * Q8_HELPERS;
+                uint32_t top = 0;                       // as bits: NaN and infinity are the largest
+#pragma unroll
+                for (int r = 0; r < LR; ++r)
+                    top = max(max(top, max(__float_as_uint(x[i][r].x) & 0x7fffffffu, __float_as_uint(x[i][r].y) & 0x7fffffffu)),
+                              max(__float_as_uint(x[i][r].z) & 0x7fffffffu, __float_as_uint(x[i][r].w) & 0x7fffffffu));
+                top = __reduce_max_sync(0xffffffffu, top);
+                float fx, gx;
+                row_exponent(__uint_as_float(top), fx, gx);
+                if (g < HEADS) {
+#pragma unroll
+                    for (int r = 0; r < LR; ++r) {
+                        const int c = lane + 32 * r;
+                        if (c < D / 4) {
+                            const float e[4] = {x[i][r].x * fx, x[i][r].y * fx, x[i][r].z * fx, x[i][r].w * fx};
+                            const uint2 hi = make_uint2(pack2<__half>(e[0], e[1]), pack2<__half>(e[2], e[3]));
+                            const int nbk = g / HB, col = SPLIT ? 2 * (g % HB) : g % HB;
+                            uint2* to = frag + ((size_t)nbk * KSTEPS + (c >> 2)) * 32 + col * 4 + (c & 3);
+                            to[0] = hi;
+                            if constexpr (SPLIT) {
+                                const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&hi.x));
+                                const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
+                                to[4] = make_uint2(pack2<__half>(e[0] - a.x, e[1] - a.y), pack2<__half>(e[2] - b.x, e[3] - b.y));
+                            }
+                        }
+                    }
+                    if (lane == 0) kf[g] = gx * p.scale * LOG2E;
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_q_full + buf * 8);
+        };
+        int4 merge = make_int4(0, 0, 0, 0);           // the unit that begins in this range and ends in a later one
+        if (w.g >= w.end) {
+            // nothing here: an empty partial, which a merge that spans this range passes over
+            for (int i = tid; i < p.GC; i += Q8_HELPERS * 32)
+                *reinterpret_cast<float2*>(p.ws_ml + ((size_t)2 * cta * p.GC + i) * 2) = make_float2(-INFINITY, 0.0f);
+        } else {
+            prepare_q(0, w);
+        }
+        for (int k = 0; w.g < w.end; ++k) {
+            const long long left = w.end - w.g;
+            const int n = (int)(left < (long long)(w.nt - w.ti) ? left : (long long)(w.nt - w.ti));
+            const bool begins = w.ti == 0, ends = w.ti + n == w.nt, whole = begins && ends;
+            const Walker u = w;
+            w.g += n - 1;
+            w.ti += n - 1;
+            walker_advance(p, w);
+            if (w.g < w.end) prepare_q(k + 1, w);
+            const int kv = u.ub / p.NCH, ch = u.ub % p.NCH;
+            const int gvalid = min(p.GC, p.G - ch * p.GC);
+            const size_t out0 = ((size_t)u.b * p.Hq + kv * p.G + ch * p.GC) * D;
+            const size_t slot = (size_t)2 * cta + (begins ? 1 : 0);
+            const int buf = k % Cfg::NF;
+            const float* s_acc = reinterpret_cast<const float*>(smem + Cfg::OFF_STATE + buf * Cfg::STATE_BYTES);
+            const float2* s_ml = reinterpret_cast<const float2*>(smem + Cfg::OFF_ML) + buf * NCW * HEADS;
+            mbar_wait(bar_state_full + buf * 8, (uint32_t)((k / Cfg::NF) & 1), abort_flag, p.status, ST_WAIT_FULL_TIMEOUT);
+            // weights of the warps' states; -1: a warp that had no tile of this segment and left no O
+            if (tid < HEADS) {
+                float m = -INFINITY, l = 0.0f;
+                float2 ml[NCW];
+#pragma unroll
+                for (int ww = 0; ww < NCW; ++ww) {
+                    ml[ww] = s_ml[ww * HEADS + tid];
+                    m = fmaxf(m, ml[ww].x);
+                }
+                const float safe = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+                for (int ww = 0; ww < NCW; ++ww) {
+                    const float f = ex2(ml[ww].x - safe);
+                    l += ml[ww].y != 0.0f ? ml[ww].y * f : 0.0f;
+                    s_w[tid * NCW + ww] = ml[ww].y != 0.0f ? f : -1.0f;
+                }
+                if (whole) l = l != 0.0f ? 1.0f / l : 0.0f;
+                else if (tid < gvalid && FTK_SLOT_OK(p, slot, 0))
+                    *reinterpret_cast<float2*>(p.ws_ml + (slot * p.GC + tid) * 2) = make_float2(m, l);
+                s_w[16 * NCW + tid] = l;
+            }
+            helpers();
+            for (int it = tid; it < gvalid * (D / 4); it += Q8_HELPERS * 32) {
+                const int g = it / (D / 4), d = (it % (D / 4)) * 4;
+                float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int ww = 0; ww < NCW; ++ww) {
+                    const float f = s_w[g * NCW + ww];
+                    float4 v = *reinterpret_cast<const float4*>(s_acc + ((size_t)ww * HEADS + g) * Cfg::ACC_STRIDE + d);
+                    if (f == -1.0f) v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    a.x = fmaf(v.x, f, a.x); a.y = fmaf(v.y, f, a.y); a.z = fmaf(v.z, f, a.z); a.w = fmaf(v.w, f, a.w);
+                }
+                if (whole) {
+                    const float inv = s_w[16 * NCW + g];
+                    store4_any(p.out, out0 + (size_t)g * D + d, p.out_dt, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
+                } else if (FTK_SLOT_OK(p, slot, 0)) {
+                    *reinterpret_cast<float4*>(p.ws_acc + (slot * p.GC + g) * D + d) = a;
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_state_empty + buf * 8);
+            helpers();                                // the weights are free again
+            if (begins && !ends) {
+                int last;
+                if (pl.ctot) last = cost_owner(pl, cost_of_unit(pl, u.b, u.ub, u.nt) + (long long)pl.ka * (u.nt - 1));
+                else last = range_of(pl, u.g + u.nt - 1);              // u stands on the unit's first tile
+                merge = make_int4(u.b, u.ub, last - cta + 1, 0);
+            }
+        }
+        if (tid == 0) p.desc[cta] = merge;
+        return;
+    }
+
     // ======================= consumer warps =======================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_CONSUMER));
     const int cg = warp / Q8_WPT, wr = warp % Q8_WPT;
     const int quad = lane >> 2, qi = lane & 3;
-    const int tc = threadIdx.x;
     const float neg_inf = -INFINITY;
-    float* s_acc = reinterpret_cast<float*>(smem + Cfg::OFF_SCRATCH);
-    float2* s_ml = reinterpret_cast<float2*>(smem + Cfg::OFF_ML);
 
-    constexpr int KSTEPS = D / 16;
     constexpr int NLD = (KSTEPS + 1) / 2;          // ldmatrix.x4 per 16 rows: two 16-byte chunks of 16 rows
-    constexpr int HB = SPLIT ? 4 : 8;              // query heads per column block
-    constexpr int HPT = SPLIT ? 1 : 2;             // of which this thread holds the scores of
+    constexpr int HPT = SPLIT ? 1 : 2;             // heads per column block that this thread holds the scores of
     uint32_t qb[NBK][KSTEPS][2];
     float acc[NBK][KSTEPS][4];                     // O^T block mt: d = 16 mt + 2 quad ([0], [1]) and + 1 ([2], [3])
     float kf[NBK][HPT];                            // score factor of the head: its row's exponent / sqrt(D) * log2(e)
@@ -460,53 +642,37 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         }
     };
 
-    int4 merge = make_int4(0, 0, 0, 0);           // the unit that begins in this range and ends in a later one
-    if (w.g >= w.end) {
-        // nothing here: an empty partial, which a merge that spans this range passes over
-        for (int i = tc; i < p.GC; i += NCW * 32)
-            *reinterpret_cast<float2*>(p.ws_ml + ((size_t)2 * cta * p.GC + i) * 2) = make_float2(neg_inf, 0.0f);
-    }
-    while (w.g < w.end) {
+    for (int k = 0; w.g < w.end; ++k) {
         const long long left = w.end - w.g;
         const int n = (int)(left < (long long)(w.nt - w.ti) ? left : (long long)(w.nt - w.ti));
-        const bool begins = w.ti == 0, ends = w.ti + n == w.nt;
-        const int kv = w.ub / p.NCH, ch = w.ub % p.NCH;
-        const int gvalid = min(p.GC, p.G - ch * p.GC);
-        const int h0 = kv * p.G + ch * p.GC;
+        const bool mine = own < i0 + n;            // this group has a tile of the segment
+        // ---- the segment's query fragments
         e0 = -1;
-        // ---- the unit's query rows as B fragments, each row scaled by a power of two into the range of a half
+        {
+            const int buf = k & 1;
+            mbar_wait(bar_q_full + buf * 8, (uint32_t)((k >> 1) & 1), abort_flag, p.status, ST_WAIT_RANGE_TIMEOUT);
+            if (mine) {
+                const uint2* frag = reinterpret_cast<const uint2*>(smem + Cfg::OFF_Q + buf * Cfg::Q_BYTES) + lane;
+                const float* s_kf = reinterpret_cast<const float*>(smem + Cfg::OFF_KF) + buf * 16;
+#pragma unroll
+                for (int nbk = 0; nbk < NBK; ++nbk) {
+#pragma unroll
+                    for (int kk = 0; kk < KSTEPS; ++kk) {
+                        const uint2 f = frag[(nbk * KSTEPS + kk) * 32];
+                        qb[nbk][kk][0] = f.x;
+                        qb[nbk][kk][1] = f.y;
+                    }
+#pragma unroll
+                    for (int e = 0; e < HPT; ++e) kf[nbk][e] = s_kf[nbk * HB + (SPLIT ? qi : 2 * qi + e)];
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_q_empty + buf * 8);
+        }
 #pragma unroll
         for (int nbk = 0; nbk < NBK; ++nbk) {
-            const int head = nbk * HB + (SPLIT ? quad >> 1 : quad);
-            float4 x[KSTEPS];
-            float top = 0.0f;
-            bool odd = false;
-#pragma unroll
-            for (int kk = 0; kk < KSTEPS; ++kk) {
-                x[kk] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (head < gvalid) x[kk] = load4_any(p.q, ((size_t)w.b * p.Hq + h0 + head) * D + kk * 16 + qi * 4, p.out_dt);
-                top = fmaxf(top, fmaxf(fmaxf(fabsf(x[kk].x), fabsf(x[kk].y)), fmaxf(fabsf(x[kk].z), fabsf(x[kk].w))));
-                odd |= (x[kk].x != x[kk].x) | (x[kk].y != x[kk].y) | (x[kk].z != x[kk].z) | (x[kk].w != x[kk].w);
-            }
-            if (odd) top = INFINITY;
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            float fx, gx;
-            row_exponent(top, fx, gx);
-            const bool rest = SPLIT && (quad & 1);
-#pragma unroll
-            for (int kk = 0; kk < KSTEPS; ++kk) {
-                float e[4] = {x[kk].x * fx, x[kk].y * fx, x[kk].z * fx, x[kk].w * fx};
-                if (rest) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) e[c] -= __half2float(__float2half_rn(e[c]));
-                }
-                qb[nbk][kk][0] = pack2<__half>(e[0], e[1]);
-                qb[nbk][kk][1] = pack2<__half>(e[2], e[3]);
-            }
 #pragma unroll
             for (int e = 0; e < HPT; ++e) {
-                kf[nbk][e] = __shfl_sync(0xffffffffu, gx, SPLIT ? 8 * qi : 4 * (2 * qi + e)) * p.scale * LOG2E;
                 m_run[nbk][e] = neg_inf;
                 l_run[nbk][e] = 0.0f;
             }
@@ -527,77 +693,42 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
             if (s >= Cfg::NS) { s -= Cfg::NS; ph ^= 1u; }
         }
         i0 += n;
-        // ---- fold the warps' states
-        const bool whole = begins && ends;
-        const float unit = e0 < 0 ? 1.0f : __uint_as_float((uint32_t)e0 << 23);      // 2^e0: sums of vs * v8 again
-        const size_t slot = (size_t)2 * cta + (begins ? 1 : 0);
+        // ---- leave the warp's state for the helpers
+        {
+            const int buf = k % Cfg::NF;
+            float* s_acc = reinterpret_cast<float*>(smem + Cfg::OFF_STATE + buf * Cfg::STATE_BYTES);
+            float2* s_ml = reinterpret_cast<float2*>(smem + Cfg::OFF_ML) + buf * NCW * HEADS;
+            const float unit = e0 < 0 ? 1.0f : __uint_as_float((uint32_t)e0 << 23);      // 2^e0: sums of vs * v8 again
+            mbar_wait(bar_state_empty + buf * 8, (uint32_t)((k / Cfg::NF) & 1) ^ 1u, abort_flag, p.status, ST_WAIT_EMPTY_TIMEOUT);
 #pragma unroll
-        for (int nbk = 0; nbk < NBK; ++nbk) {
-            bar_consumers();                       // scratch is free again
+            for (int nbk = 0; nbk < NBK; ++nbk) {
 #pragma unroll
-            for (int e = 0; e < HPT; ++e) {
-                float l = l_run[nbk][e];
-                l += __shfl_xor_sync(0xffffffffu, l, 4);
-                l += __shfl_xor_sync(0xffffffffu, l, 8);
-                l += __shfl_xor_sync(0xffffffffu, l, 16);
-                const float m = m_run[nbk][e];
-                const int g = SPLIT ? qi : qi * 2 + e;
-                float* my = s_acc + ((size_t)warp * 8 + g) * Cfg::ACC_STRIDE + quad * 2;
+                for (int e = 0; e < HPT; ++e) {
+                    float l = l_run[nbk][e];
+                    l += __shfl_xor_sync(0xffffffffu, l, 4);
+                    l += __shfl_xor_sync(0xffffffffu, l, 8);
+                    l += __shfl_xor_sync(0xffffffffu, l, 16);
+                    const int g = nbk * HB + (SPLIT ? qi : qi * 2 + e);
+                    if (quad == 0) s_ml[warp * HEADS + g] = make_float2(m_run[nbk][e], l);
+                    if (e0 >= 0) {
+                        float* my = s_acc + ((size_t)warp * HEADS + g) * Cfg::ACC_STRIDE + quad * 2;
 #pragma unroll
-                for (int mt = 0; mt < KSTEPS; ++mt) {
-                    float2 o;
-                    if constexpr (SPLIT) o = make_float2(acc[nbk][mt][0] + acc[nbk][mt][1], acc[nbk][mt][2] + acc[nbk][mt][3]);
-                    else o = make_float2(acc[nbk][mt][e], acc[nbk][mt][2 + e]);
-                    *reinterpret_cast<float2*>(my + mt * 16) = make_float2(o.x * unit, o.y * unit);
-                }
-                if (quad == 0) s_ml[warp * 8 + g] = make_float2(m, l);
-            }
-            bar_consumers();
-            for (int it = tc; it < HB * (D / 2); it += NCW * 32) {
-                const int row = it / (D / 2), d = (it % (D / 2)) * 2;
-                const int g = nbk * HB + row;
-                if (g >= gvalid) continue;
-                float mw[NCW];
-                float mg = neg_inf;
-#pragma unroll
-                for (int ww = 0; ww < NCW; ++ww) {
-                    mw[ww] = s_ml[ww * 8 + row].x;
-                    mg = fmaxf(mg, mw[ww]);
-                }
-                const float mg_safe = mg == neg_inf ? 0.0f : mg;
-                float a0 = 0.0f, a1 = 0.0f, lg = 0.0f;
-#pragma unroll
-                for (int ww = 0; ww < NCW; ++ww) {
-                    const float sc = ex2(mw[ww] - mg_safe);
-                    const float2 v = *reinterpret_cast<const float2*>(s_acc + ((size_t)ww * 8 + row) * Cfg::ACC_STRIDE + d);
-                    a0 += v.x * sc;
-                    a1 += v.y * sc;
-                    lg += s_ml[ww * 8 + row].y * sc;
-                }
-                if (whole) {
-                    const float inv = lg != 0.0f ? 1.0f / lg : 0.0f;
-                    store2_any(p.out, ((size_t)w.b * p.Hq + h0 + g) * D + d, p.out_dt, a0 * inv, a1 * inv);
-                } else if (FTK_SLOT_OK(p, slot, 0)) {
-                    const size_t pr = slot * p.GC + g;
-                    *reinterpret_cast<float2*>(p.ws_acc + pr * D + d) = make_float2(a0, a1);
-                    if (d == 0) *reinterpret_cast<float2*>(p.ws_ml + pr * 2) = make_float2(mg, lg);
+                        for (int mt = 0; mt < KSTEPS; ++mt) {
+                            float2 o;
+                            if constexpr (SPLIT) o = make_float2(acc[nbk][mt][0] + acc[nbk][mt][1], acc[nbk][mt][2] + acc[nbk][mt][3]);
+                            else o = make_float2(acc[nbk][mt][e], acc[nbk][mt][2 + e]);
+                            *reinterpret_cast<float2*>(my + mt * 16) = make_float2(o.x * unit, o.y * unit);
+                        }
+                    }
                 }
             }
-        }
-        if (begins && !ends) {
-            int last;
-            if (pl.ctot) {
-                last = cost_owner(pl, cost_of_unit(pl, w.b, w.ub, w.nt) + (long long)pl.ka * (w.nt - 1));
-            } else {
-                last = range_of(pl, w.g + w.nt - 1);              // w stands on the unit's first tile
-            }
-            merge = make_int4(w.b, w.ub, last - cta + 1, 0);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_state_full + buf * 8);
         }
         w.g += n - 1;
         w.ti += n - 1;
         walker_advance(p, w);
     }
-    if (tc == 0) p.desc[cta] = merge;
 }
 
 // ---- generic kernel ---------------------------------------------------------------
@@ -750,14 +881,15 @@ decode_q8_generic_kernel(const Q8Params p) {
 // ---- merge -------------------------------------------------------------------------
 // Folds the partials of the units that were cut. TC: block c looks at the unit that begins in range c of the tensor-core
 // kernel and ends in a later one, if any: its first partial is slot 2 c + 1, the next ones the even slots behind.
-// Otherwise block u folds the nsplit slots of unit u of the generic kernel. Weights 2^(m_j - max m) worked out once per
-// (partial, head) in shared memory; the sums run over the partials in order, four float4 loads in flight per thread.
-constexpr int Q8M_THREADS = 128;
-constexpr int Q8M_ROUND = 1024;                     // (partial, head) weights per round
+// Otherwise block u folds the nsplit slots of unit u of the generic kernel. All latency: the (m, l) of up to 32 partials and
+// the first sums of each thread's are requested together; 4 teams of threads take every fourth partial, and their sums
+// are added in order.
+constexpr int Q8M_TEAMS = 4, Q8M_TEAM = 128, Q8M_THREADS = Q8M_TEAMS * Q8M_TEAM;
 template <bool TC>
 __global__ void __launch_bounds__(Q8M_THREADS) q8_merge_kernel(const Q8Params p) {
-    __shared__ float s_w[Q8M_ROUND];
-    __shared__ float s_top[16], s_l[16];
+    __shared__ float s_w[16][32];                   // weights of a round of 32 partials; -1: empty, its sums unwritten
+    __shared__ float s_top[16], s_l[16], s_scale[16];
+    __shared__ float4 s_sum[Q8M_TEAMS - 1][Q8M_TEAM];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int c = (int)blockIdx.x, tid = threadIdx.x;
@@ -774,54 +906,71 @@ __global__ void __launch_bounds__(Q8M_THREADS) q8_merge_kernel(const Q8Params p)
     const int kv = ub / p.NCH, ch = ub % p.NCH;
     const int gv = min(p.GC, p.G - ch * p.GC);
     const int h0 = kv * p.G + ch * p.GC;
-    // the largest exponent of each head, a warp per head
     const int warp = tid >> 5, lane = tid & 31;
-    for (int g = warp; g < gv; g += Q8M_THREADS / 32) {
-        float top = -INFINITY;
-        for (int j = lane; j < parts; j += 32) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml + (slot(j) * p.GC + g) * 2));
-            if (ml.y != 0.0f) top = fmaxf(top, ml.x);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (top == -INFINITY) top = 0.0f;
-        float sum = 0.0f;
-        for (int j = lane; j < parts; j += 32) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml + (slot(j) * p.GC + g) * 2));
-            if (ml.y != 0.0f) sum += ml.y * ex2(ml.x - top);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) { s_top[g] = top; s_l[g] = sum; }
-    }
+    const int team = tid / Q8M_TEAM, at = tid % Q8M_TEAM;
     const int quads = p.D >> 2, items = gv * quads;
-    const int round = Q8M_ROUND / gv;
-    for (int i0 = 0; i0 < items; i0 += Q8M_THREADS) {
-        const int it = i0 + tid;
+    if (tid < 16) { s_top[tid] = -INFINITY; s_l[tid] = 0.0f; }
+    for (int i0 = 0; i0 < items; i0 += Q8M_TEAM) {
+        const int it = i0 + at;
         const int g = it < items ? it / quads : 0, d = it < items ? (it - g * quads) * 4 : 0;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int j0 = 0; j0 < parts; j0 += round) {
-            const int n = min(round, parts - j0);
-            if (i0 == 0 || parts > round) {
-                __syncthreads();
-                for (int k = tid; k < n * gv; k += Q8M_THREADS) {
-                    const int gg = k % gv;
-                    const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml + (slot(j0 + k / gv) * p.GC + gg) * 2));
-                    s_w[k] = ml.y != 0.0f ? ex2(ml.x - s_top[gg]) : -1.0f;         // -1: an empty partial, its sums unwritten
-                }
-                __syncthreads();
+        for (int j0 = 0; j0 < parts; j0 += 32) {
+            const int n = min(32, parts - j0);
+            __syncthreads();
+            // every fourth partial of the round, requested before anything is known about the weights (an empty one's slot
+            // is allocated, its contents are not used)
+            float4 v[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const int j = team + Q8M_TEAMS * q;
+                v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (it < items && j < n) v[q] = __ldcg(reinterpret_cast<const float4*>(p.ws_acc + (slot(j0 + j) * p.GC + g) * p.D + d));
             }
-            if (it < items) {
-#pragma unroll 4
-                for (int j = 0; j < n; ++j) {
-                    const float f = s_w[j * gv + g];
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (f >= 0.0f || f != f) v = __ldcg(reinterpret_cast<const float4*>(p.ws_acc + (slot(j0 + j) * p.GC + g) * p.D + d));
-                    a.x = fmaf(v.x, f, a.x); a.y = fmaf(v.y, f, a.y); a.z = fmaf(v.z, f, a.z); a.w = fmaf(v.w, f, a.w);
+            if (i0 == 0 || parts > 32) {
+                for (int gg = warp; gg < gv; gg += Q8M_THREADS / 32) {
+                    float2 ml = make_float2(-INFINITY, 0.0f);
+                    if (lane < n) ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml + (slot(j0 + lane) * p.GC + gg) * 2));
+                    const float before = j0 ? s_top[gg] : -INFINITY;
+                    float now = ml.y != 0.0f ? ml.x : -INFINITY;
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
+                    now = fmaxf(now, before);
+                    const float safe = now == -INFINITY ? 0.0f : now;
+                    const float f = ex2(ml.x - safe);
+                    s_w[gg][lane] = ml.y != 0.0f ? f : -1.0f;
+                    float sum = ml.y != 0.0f ? ml.y * f : 0.0f;
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    if (lane == 0) {
+                        s_scale[gg] = ex2(before - safe);
+                        s_l[gg] = (j0 ? s_l[gg] * s_scale[gg] : 0.0f) + sum;
+                        s_top[gg] = now;
+                    }
+                    __syncwarp();
                 }
+            }
+            __syncthreads();
+            if (j0) {
+                const float r = s_scale[g];
+                a.x *= r; a.y *= r; a.z *= r; a.w *= r;
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const int j = team + Q8M_TEAMS * q;
+                if (j >= n) break;
+                const float f = s_w[g][j];
+                if (f == -1.0f) continue;
+                a.x = fmaf(v[q].x, f, a.x); a.y = fmaf(v[q].y, f, a.y); a.z = fmaf(v[q].z, f, a.z); a.w = fmaf(v[q].w, f, a.w);
             }
         }
-        if (it < items) {
+        if (team) s_sum[team - 1][at] = a;
+        __syncthreads();
+        if (!team && it < items) {
+#pragma unroll
+            for (int t = 0; t < Q8M_TEAMS - 1; ++t) {
+                const float4 v = s_sum[t][at];
+                a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+            }
             const float l = s_l[g];
             const float inv = l != 0.0f ? 1.0f / l : 0.0f;
             store4_any(p.out, ((size_t)b * p.Hq + h0 + g) * p.D + d, p.out_dt, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));

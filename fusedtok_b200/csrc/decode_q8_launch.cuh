@@ -10,12 +10,12 @@ template <typename KV, int D, int NBK, bool SPLIT>
 cudaError_t q8_launch_one(const CUtensorMap& mk, const CUtensorMap& mv, const Q8Params& p, cudaStream_t cs) {
     // a function attribute, not a stream operation: cheap, and legal while the stream is captured
     cudaError_t e = cudaFuncSetAttribute(decode_q8_kernel<KV, D, NBK, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         Q8Cfg<D>::SMEM_BYTES);
+                                         (Q8Cfg<D, NBK, SPLIT>::SMEM_BYTES));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.ncta);
-    cfg.blockDim = dim3(TC_THREADS);
-    cfg.dynamicSmemBytes = Q8Cfg<D>::SMEM_BYTES;
+    cfg.blockDim = dim3(Q8_THREADS);
+    cfg.dynamicSmemBytes = (Q8Cfg<D, NBK, SPLIT>::SMEM_BYTES);
     cfg.stream = cs;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -283,21 +283,34 @@ int fusedtok_kv_append_paged_q8_launch(int dtype, int store, const void* k_new, 
     p.scales = kv_scales; p.slots = slots;
     p.N = tokens; p.Hkv = kv_heads; p.D = dim; p.page = page;
     p.rows = num_blocks * page;
-    // a token per CTA while that fills the GPU no more than a few times over, up to a block's worth beyond
-    const long long ctas = (long long)tokens * kv_heads * 2;
-    p.window = (int)std::max<long long>(1, std::min<long long>({ctas / (16ll * sms), (long long)page, (long long)AQ_THREADS}));
-    const dim3 grid((unsigned)((tokens + p.window - 1) / p.window), (unsigned)kv_heads, 2);
     const bool wide = es == 2 && dim % 8 == 0 && (news & 15u) == 0 && (pools & 7u) == 0;
+    // a warp where it can hold a block's rows in its registers, else a CTA of four
+    const int vec = wide ? 8 : 4;
+    const int team = (long long)page * dim <= 32ll * AQ_HELD * vec ? 32 : AQ_THREADS;
+    // a token per team while all teams are resident at once, up to a block's worth of tokens beyond
+    const long long heads = 2ll * kv_heads;
+    const long long resident = (long long)sms * (team == 32 ? 20 : 5);
+    p.window = (int)std::max<long long>(1, std::min<long long>({tokens * heads / resident, (long long)page, (long long)team}));
+    p.windows = (tokens + p.window - 1) / p.window;
+    const long long ctas = (p.windows * heads + AQ_THREADS / team - 1) / (AQ_THREADS / team);
+    if (ctas > 0x7fffffffll) return fail(FUSEDTOK_INVALID_ARGUMENT, "too many tokens and heads for one launch");
+    const dim3 grid((unsigned)ctas);
     cudaStream_t cs = (cudaStream_t)stream;
     const char* what = "8-bit kv append kernel launch";
-#define FTK_GO(T, V)                                                                                            \
-    return store == 0 ? launch_pdl(kv_append_q8_kernel<T, int8_t, V>, grid, dim3(AQ_THREADS), 0, cs, p, what)   \
-                      : launch_pdl(kv_append_q8_kernel<T, __nv_fp8_e4m3, V>, grid, dim3(AQ_THREADS), 0, cs, p, what)
+#define FTK_TEAM(T, KV, V) \
+    return team == 32 ? launch_pdl(kv_append_q8_kernel<T, KV, V, 32>, grid, dim3(AQ_THREADS), 0, cs, p, what) \
+                      : launch_pdl(kv_append_q8_kernel<T, KV, V, AQ_THREADS>, grid, dim3(AQ_THREADS), 0, cs, p, what)
+#define FTK_GO(T, V)                                  \
+    do {                                              \
+        if (store == 0) FTK_TEAM(T, int8_t, V);       \
+        FTK_TEAM(T, __nv_fp8_e4m3, V);                \
+    } while (0)
     if (dtype == 0) FTK_GO(float, 4);
     if (dtype == 1) { if (wide) FTK_GO(__nv_bfloat16, 8); FTK_GO(__nv_bfloat16, 4); }
     if (wide) FTK_GO(__half, 8);
     FTK_GO(__half, 4);
 #undef FTK_GO
+#undef FTK_TEAM
 }
 
 int fusedtok_block_table_extend_launch(int* table, const int* lens, const int* new_lens, const int* free_blocks,

@@ -553,17 +553,35 @@ def rope_kv_append_paged(q, k_pool, v_pool, block_table, k_new, v_new, lens, *, 
 
 # code type of the pools -> store code of the C ABI
 _CODES = {} if torch is None else {torch.int8: 0, torch.float8_e4m3fn: 1}
-_q8_workspace = {}       # (device, shape) -> bytes of workspace the launcher asks for
+_INT32 = None if torch is None else torch.int32
+_FLOAT32 = None if torch is None else torch.float32
+_q8_workspace = {}       # (device index, shape) -> floats of workspace the launcher asks for
+_device_now = getattr(getattr(torch, "_C", None), "_cuda_getDevice", None)
 
 
-def _q8_operands(lead, k_pool, v_pool, kv_scales, **rest):
-    """Checks common to the operators on an 8-bit paged cache: activations `rest` of one storage type, pools of one
-    code type, float32 scales, everything contiguous on one device. Returns (call, store, Nb, Hkv, P, D)."""
-    if not _on_gpu(lead):
-        raise TypeError("the operators on an 8-bit cache work on CUDA tensors only")
-    call = _DeviceCall(**rest)
-    for name, t, allowed in (("k_pool", k_pool, _CODES), ("v_pool", v_pool, _CODES),
-                             ("kv_scales", kv_scales, (torch.float32,))):
+def _ready(index, dtype, *tensors):
+    """True if all are contiguous tensors of `dtype` on CUDA device `index`: the quick look that the calls of a decode
+    loop pass. Where it fails, the careful checks find out why."""
+    for t in tensors:
+        if not (isinstance(t, _Tensor) and t.dtype is dtype and t.get_device() == index and t.is_contiguous()):
+            return False
+    return index >= 0
+
+
+def _run(index, fn, *args):
+    """`fn(*args, stream)` of the C ABI on the current stream of device `index`, its status raised as an exception."""
+    if _raw_stream is None or (_device_now() if _device_now is not None else -1) != index:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    else:
+        rc = fn(*args, _raw_stream(index))
+    if rc:
+        _fusedtok._check(rc)
+
+
+def _q8_cache(call, k_pool, v_pool, kv_scales):
+    """Raise what is wrong with the cache operands of a call (the activations are checked: `call`)."""
+    for name, t, allowed in (("k_pool", k_pool, _CODES), ("v_pool", v_pool, _CODES), ("kv_scales", kv_scales, (_FLOAT32,))):
         if not _on_gpu(t):
             raise TypeError(f"{name}: a CUDA tensor is required")
         if t.dtype not in allowed:
@@ -575,16 +593,21 @@ def _q8_operands(lead, k_pool, v_pool, kv_scales, **rest):
             raise ValueError(f"{name}: a contiguous tensor is required")
     if v_pool.dtype is not k_pool.dtype:
         raise TypeError(f"v_pool: dtype {v_pool.dtype} differs from k_pool's {k_pool.dtype}")
-    if k_pool.ndim != 4:
-        raise ValueError(f"k_pool: {k_pool.ndim}-D tensor where [Nb, Hkv, P, D] is expected")
-    if v_pool.shape != k_pool.shape:
-        raise ValueError(f"v_pool: shape {tuple(v_pool.shape)} differs from k_pool's {tuple(k_pool.shape)}")
-    blocks, hkv, page, dim = k_pool.shape
+
+
+def _q8_shape(k_pool, v_pool, kv_scales):
+    """(Nb, Hkv, P, D) of an 8-bit cache whose shapes agree."""
+    shape = k_pool.shape
+    if len(shape) != 4:
+        raise ValueError(f"k_pool: {len(shape)}-D tensor where [Nb, Hkv, P, D] is expected")
+    if v_pool.shape != shape:
+        raise ValueError(f"v_pool: shape {tuple(v_pool.shape)} differs from k_pool's {tuple(shape)}")
+    blocks, hkv, page, dim = shape
     if kv_scales.shape != (blocks, hkv, 2):
         raise ValueError(f"kv_scales: shape {tuple(kv_scales.shape)} where {(blocks, hkv, 2)} follows from the pools")
     if page < 1:
         raise ValueError("k_pool: blocks of at least one row are required")
-    return call, _CODES[k_pool.dtype], blocks, hkv, page, dim
+    return blocks, hkv, page, dim
 
 
 def attention_decode_paged_q8(q, k_pool, v_pool, kv_scales, block_table, lens=None):
@@ -595,29 +618,48 @@ def attention_decode_paged_q8(q, k_pool, v_pool, kv_scales, block_table, lens=No
     q ``[B, Hq, D]`` float32, bfloat16 or float16 (the result has its type, accumulation is float32); pools
     ``[Nb, Hkv, P, D]`` of ``torch.int8`` or ``torch.float8_e4m3fn`` codes; kv_scales ``[Nb, Hkv, 2]`` float32: K's
     scale, then V's (``kv_append_paged_q8`` fills both); block_table ``[B, S]`` and lens ``[B]`` as in
-    ``attention_decode_paged``. Any GQA group. CUDA tensors only; host table and lens values are checked, CUDA
-    tensors trusted. The scratch of a call comes from torch's allocator, so calls on different streams do not share
-    any. No counterpart in the reference."""
-    call, store, blocks, hkv, page, dim = _q8_operands(q, k_pool, v_pool, kv_scales, q=q)
-    b, hq, d = call.dims("q", "B Hq D")
+    ``attention_decode_paged``. Any GQA group. The V scales of one sequence's blocks may differ by a factor of up to
+    2^60. CUDA tensors only; host table and lens values are checked, CUDA tensors trusted. The scratch of a call comes
+    from torch's allocator, so calls on different streams do not share any. No counterpart in the reference."""
+    index = q.get_device() if isinstance(q, _Tensor) else -1
+    given = (block_table,) if lens is None else (block_table, lens)
+    host = None
+    if not (q.dtype in _STORAGE and _ready(index, q.dtype, q) and getattr(k_pool, "dtype", None) in _CODES
+            and _ready(index, k_pool.dtype, k_pool, v_pool) and _ready(index, _FLOAT32, kv_scales)
+            and _ready(index, _INT32, *given)) if index >= 0 else True:
+        if not _on_gpu(q):
+            raise TypeError("the operators on an 8-bit cache work on CUDA tensors only")
+        host = _DeviceCall(q=q)
+        _q8_cache(host, k_pool, v_pool, kv_scales)
+    blocks, hkv, page, dim = _q8_shape(k_pool, v_pool, kv_scales)
+    if len(q.shape) != 3:
+        raise ValueError(f"q: {len(q.shape)}-D tensor where [B, Hq, D] is expected")
+    b, hq, d = q.shape
     if d != dim:
         raise ValueError(f"k_pool: head dim {dim} differs from q's {d}")
     _gqa_heads(hq, hkv)
-    table = call.index("block_table", block_table, (b, None), blocks, False)
-    width = table.shape[1]
-    lens_dev = None if lens is None else call.index("lens", lens, (b,), width * page, True)
-    out = call.new((b, hq, d))
+    if host is not None:
+        block_table = host.index("block_table", block_table, (b, None), blocks, False)
+        if lens is not None:
+            lens = host.index("lens", lens, (b,), block_table.shape[1] * page, True)
+    else:
+        _index_shape("block_table", block_table.shape, (b, None))
+        if lens is not None:
+            _index_shape("lens", lens.shape, (b,))
+    width = block_table.shape[1]
+    out = torch.empty_like(q)
     if b:
-        key = (call.device, call.code, b, hq, hkv, page, width, d)
-        need = _q8_workspace.get(key)
-        if need is None:
-            with torch.cuda.device(call.device):
-                need = _q8_workspace[key] = _fusedtok.attention_decode_paged_q8_workspace(*key[1:])
-        scratch = torch.empty(need, dtype=torch.uint8, device=call.device)
-        call.launch(_fusedtok.attention_decode_paged_q8_launch, call.code, store, q.data_ptr(), k_pool.data_ptr(),
-                    v_pool.data_ptr(), kv_scales.data_ptr(), table.data_ptr(),
-                    None if lens_dev is None else lens_dev.data_ptr(), out.data_ptr(), scratch.data_ptr(), need, b, hq,
-                    hkv, page, width, blocks, d)
+        code = _STORAGE[q.dtype][1]
+        key = (index, code, b, hq, hkv, page, width, d)
+        floats = _q8_workspace.get(key)
+        if floats is None:
+            with torch.cuda.device(index):
+                floats = _q8_workspace[key] = (_fusedtok.attention_decode_paged_q8_workspace(*key[1:]) + 3) // 4
+        scratch = kv_scales.new_empty(floats)
+        _run(index, _fusedtok._lib.fusedtok_attention_decode_paged_q8_launch, code, _CODES[k_pool.dtype], q.data_ptr(),
+             k_pool.data_ptr(), v_pool.data_ptr(), kv_scales.data_ptr(), block_table.data_ptr(),
+             None if lens is None else lens.data_ptr(), out.data_ptr(), scratch.data_ptr(), 4 * floats, b, hq, hkv, page,
+             width, blocks, d)
     return out
 
 
@@ -633,20 +675,35 @@ def kv_append_paged_q8(k_pool, v_pool, kv_scales, k_new, v_new, slots):
     A value that is not finite makes the block's scale NaN. CUDA tensors only; host slots are checked (``< Nb * P``,
     and the rule above), a CUDA tensor is trusted (slots outside the pool are passed over). No counterpart in the
     reference."""
-    call, store, blocks, hkv, page, dim = _q8_operands(k_pool, k_pool, v_pool, kv_scales, k_new=k_new, v_new=v_new)
-    n, nh, nd = call.dims("k_new", "N Hkv D")
-    call.same_shape("v_new", "k_new")
-    if (nh, nd) != (hkv, dim):
+    index = k_pool.get_device() if isinstance(k_pool, _Tensor) else -1
+    call = None
+    if not (isinstance(k_new, _Tensor) and k_new.dtype in _STORAGE and _ready(index, k_new.dtype, k_new, v_new)
+            and k_pool.dtype in _CODES and _ready(index, k_pool.dtype, k_pool, v_pool)
+            and _ready(index, _FLOAT32, kv_scales) and _ready(index, _INT32, slots)):
+        if not _on_gpu(k_pool):
+            raise TypeError("the operators on an 8-bit cache work on CUDA tensors only")
+        call = _DeviceCall(k_new=k_new, v_new=v_new)
+        _q8_cache(call, k_pool, v_pool, kv_scales)
+    blocks, hkv, page, dim = _q8_shape(k_pool, v_pool, kv_scales)
+    if len(k_new.shape) != 3:
+        raise ValueError(f"k_new: {len(k_new.shape)}-D tensor where [N, Hkv, D] is expected")
+    if v_new.shape != k_new.shape:
+        raise ValueError(f"v_new: shape {tuple(v_new.shape)} differs from k_new's {tuple(k_new.shape)}")
+    n, nh, nd = k_new.shape
+    if nh != hkv or nd != dim:
         raise ValueError(f"k_new: [Hkv, D] = {(nh, nd)} differs from the cache's {(hkv, dim)}")
     if blocks * page > 0x7fffffff:
         raise ValueError(f"k_pool: {blocks} blocks of {page} rows are more rows than a slot can name")
-    if not _on_gpu(slots):
-        slots = _host_slots(slots, n, blocks, page)
-    where = call.index("slots", slots, (n,), blocks * page, False) if _on_gpu(slots) else torch.from_numpy(slots).to(call.device)
+    if call is None:
+        _index_shape("slots", slots.shape, (n,))
+    elif _on_gpu(slots):
+        slots = call.index("slots", slots, (n,), blocks * page, False)
+    else:
+        slots = torch.from_numpy(_host_slots(slots, n, blocks, page)).to(call.device)
     if n:
-        call.launch(_fusedtok.kv_append_paged_q8_launch, call.code, store, k_new.data_ptr(), v_new.data_ptr(),
-                    where.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), kv_scales.data_ptr(), n, hkv, dim, page,
-                    blocks)
+        _run(index, _fusedtok._lib.fusedtok_kv_append_paged_q8_launch, _STORAGE[k_new.dtype][1], _CODES[k_pool.dtype],
+             k_new.data_ptr(), v_new.data_ptr(), slots.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
+             kv_scales.data_ptr(), n, hkv, dim, page, blocks)
     return None
 
 
@@ -682,21 +739,28 @@ class BlockTableStep(NamedTuple):
     free_count: object
 
 
-def _table_operands(block_table, page, **rest):
-    """Operands of the block table operators: contiguous int32 CUDA tensors of one device (they hold the state of the
-    cache, so nothing is converted). Returns (call, B, S)."""
-    if not _on_gpu(block_table):
-        raise TypeError("the block table operators work on CUDA tensors only")
-    call = _DeviceCall(dtypes=(torch.int32,), block_table=block_table, **rest)
-    b, width = call.dims("block_table", "B S")
-    for name in ("lens", "new_lens", "keep_lens"):
-        if name in rest:
-            _index_shape(name, rest[name].shape, (b,))
-    _index_shape("free_blocks", rest["free_blocks"].shape, (None,))
-    _index_shape("free_count", rest["free_count"].shape, (1,))
+def _table_operands(page, block_table, lens, change, free_blocks, free_count, change_name):
+    """Check the operands of a block table operator: contiguous int32 CUDA tensors of one device (they hold the state of
+    the cache, so nothing is converted). Returns (device index, B, S)."""
+    index = block_table.get_device() if isinstance(block_table, _Tensor) else -1
+    if not _ready(index, _INT32, block_table, lens, change, free_blocks, free_count):
+        if not _on_gpu(block_table):
+            raise TypeError("the block table operators work on CUDA tensors only")
+        _DeviceCall(dtypes=(_INT32,), **{"block_table": block_table, "lens": lens, change_name: change,
+                                         "free_blocks": free_blocks, "free_count": free_count})
+    _index_shape("block_table", block_table.shape, (None, None))
+    b, width = block_table.shape
+    if lens.shape != (b,):
+        _index_shape("lens", lens.shape, (b,))
+    if change.shape != (b,):
+        _index_shape(change_name, change.shape, (b,))
+    if len(free_blocks.shape) != 1:
+        _index_shape("free_blocks", free_blocks.shape, (None,))
+    if free_count.shape != (1,):
+        _index_shape("free_count", free_count.shape, (1,))
     if int(page) != page or page < 1:
         raise ValueError(f"page {page}: blocks of at least one row are required")
-    return call, b, width
+    return index, b, width
 
 
 def block_table_extend(block_table, lens, new_lens, free_blocks, free_count, page, max_tokens):
@@ -711,15 +775,17 @@ def block_table_extend(block_table, lens, new_lens, free_blocks, free_count, pag
     get slot -1. So is the first one that the free stack cannot serve, and every later one that needs a block. All
     tensors are contiguous int32 CUDA tensors (at most 8192 sequences), read on the GPU and trusted; free_blocks and
     free_count are not changed - give the returned count to the next call. No counterpart in the reference."""
-    call, b, width = _table_operands(block_table, page, lens=lens, new_lens=new_lens, free_blocks=free_blocks,
-                                     free_count=free_count)
+    index, b, width = _table_operands(page, block_table, lens, new_lens, free_blocks, free_count, "new_lens")
     if int(max_tokens) != max_tokens or not 0 <= max_tokens <= 0x7fffffff:
         raise ValueError(f"max_tokens {max_tokens}: a count of tokens below 2^31 is expected")
-    slots, starts, lens_out, left = (call.new((k,)) for k in (int(max_tokens), b + 1, b, 1))
-    call.launch(_fusedtok.block_table_extend_launch, block_table.data_ptr(), lens.data_ptr(), new_lens.data_ptr(),
-                free_blocks.data_ptr(), free_count.data_ptr(), slots.data_ptr(), starts.data_ptr(),
-                lens_out.data_ptr(), left.data_ptr(), b, width, int(page), free_blocks.shape[0], int(max_tokens))
-    return BlockTableStep(slots, starts, lens_out, left)
+    n = int(max_tokens)
+    made = lens.new_empty(n + 2 * b + 2)                 # one allocation for the four results
+    step = BlockTableStep(*made.split_with_sizes([n, b + 1, b, 1]))
+    at = made.data_ptr()
+    _run(index, _fusedtok._lib.fusedtok_block_table_extend_launch, block_table.data_ptr(), lens.data_ptr(),
+         new_lens.data_ptr(), free_blocks.data_ptr(), free_count.data_ptr(), at, at + 4 * n, at + 4 * (n + b + 1),
+         at + 4 * (n + 2 * b + 1), b, width, int(page), free_blocks.shape[0], n)
+    return step
 
 
 def block_table_trim(block_table, lens, keep_lens, free_blocks, free_count, page):
@@ -727,10 +793,9 @@ def block_table_trim(block_table, lens, keep_lens, free_blocks, free_count, page
     tokens) and push the blocks that they no longer need on the free stack, in batch order, from
     ``free_blocks[free_count]`` on. Returns ``(lens, free_count)``, the new lengths and count; the table is only read.
     Operands as in :func:`block_table_extend`. No counterpart in the reference."""
-    call, b, width = _table_operands(block_table, page, lens=lens, keep_lens=keep_lens, free_blocks=free_blocks,
-                                     free_count=free_count)
-    lens_out, left = call.new((b,)), call.new((1,))
-    call.launch(_fusedtok.block_table_trim_launch, block_table.data_ptr(), lens.data_ptr(), keep_lens.data_ptr(),
-                free_blocks.data_ptr(), free_count.data_ptr(), lens_out.data_ptr(), left.data_ptr(), b, width,
-                int(page), free_blocks.shape[0])
+    index, b, width = _table_operands(page, block_table, lens, keep_lens, free_blocks, free_count, "keep_lens")
+    lens_out, left = lens.new_empty(b), lens.new_empty(1)
+    _run(index, _fusedtok._lib.fusedtok_block_table_trim_launch, block_table.data_ptr(), lens.data_ptr(),
+         keep_lens.data_ptr(), free_blocks.data_ptr(), free_count.data_ptr(), lens_out.data_ptr(), left.data_ptr(), b,
+         width, int(page), free_blocks.shape[0])
     return lens_out, left

@@ -8,9 +8,9 @@
 // trim: the blocks behind ceil(keep / P) go back, in batch order, to free[free_count], free[free_count + 1], ...
 //
 // A few hundred bytes to a megabyte move; what counts is latency. One launch each: every CTA works out the prefix sums
-// of the whole batch for itself in shared memory (up to BT_MAX_BATCH sequences, two block-wide scans per BT_THREADS
-// sequences), which spares a second launch or a barrier across the grid, and then takes its share of the outputs: a warp
-// per sequence for table entries, a thread per 4 tokens for slots, the token's sequence found by binary search.
+// of the whole batch for itself in shared memory (up to BT_MAX_BATCH sequences, one block-wide scan of two sums per
+// BT_THREADS sequences), which spares a second launch or a barrier across the grid, and then takes its share of the
+// outputs, counted in table entries and slots: whose they are is found by binary search in the sums.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -34,112 +34,128 @@ struct BlockTableParams {
     int B, width, page, capacity, max_tokens;
 };
 
-// Inclusive sum over the block of one value per thread; `total` gets the sum of all.
-__device__ __forceinline__ long long bt_scan(long long v, long long* red, long long& total) {
+struct Sums {
+    long long a, b;
+};
+// Inclusive sums over the block of two values per thread; `total` gets the sums of all.
+__device__ __forceinline__ Sums bt_scan(Sums v, Sums* red, Sums& total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long t = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += t;
+        const long long a = __shfl_up_sync(0xffffffffu, v.a, o), b = __shfl_up_sync(0xffffffffu, v.b, o);
+        if (lane >= o) { v.a += a; v.b += b; }
     }
     __syncthreads();                                   // red is free again
     if (lane == 31) red[warp] = v;
     __syncthreads();
-    total = 0;
+    total = Sums{0, 0};
 #pragma unroll
     for (int w = 0; w < BT_THREADS / 32; ++w) {
-        if (w < warp) v += red[w];
-        total += red[w];
+        const Sums t = red[w];
+        if (w < warp) { v.a += t.a; v.b += t.b; }
+        total.a += t.a;
+        total.b += t.b;
     }
     return v;
 }
-__device__ __forceinline__ int bt_blocks(long long tokens, int page) { return (int)((tokens + page - 1) / page); }
+__device__ __forceinline__ int bt_blocks(long long tokens, int page) {
+    return (int)((unsigned)(tokens + page - 1) / (unsigned)page);      // (tokens + page < 2^32: both are below 2^31)
+}
+// last index in [0, n) whose sum is at most x (the sums do not decrease, s[0] <= x); the top bit of an entry is a flag
+__device__ __forceinline__ int bt_find(const int* s, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if ((s[mid] & 0x7fffffff) <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+constexpr int BT_REFUSED = (int)0x80000000;
 
 __global__ void __launch_bounds__(BT_THREADS) block_table_extend_kernel(const BlockTableParams p) {
     extern __shared__ int bt_smem[];
-    int* s_end = bt_smem;                              // [B] tokens up to and including b's (INT_MAX at most)
-    int* s_off = bt_smem + p.B;                        // [B] blocks asked for before b's; -1: refused
-    __shared__ long long red[BT_THREADS / 32];
+    int* s_start = bt_smem;                            // [B + 1] tokens before b's (2^31 - 1 at most)
+    int* s_off = bt_smem + p.B + 1;                    // [B] blocks asked for before b's; BT_REFUSED: none for b
+    __shared__ Sums red[BT_THREADS / 32];
+    __shared__ int s_taken;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x;
     const long long room = (long long)p.width * p.page;
     const int count = min(max(__ldg(p.free_count), 0), p.capacity);
-    long long tokens = 0, asked = 0, taken = 0;
+    if (tid == 0) { s_taken = 0; s_start[0] = 0; }
+    long long tokens = 0, asked = 0;
     for (int base = 0; base < p.B; base += BT_THREADS) {
         const int b = base + tid;
         const long long len = b < p.B ? max(__ldg(p.lens + b), 0) : 0;
         const long long add = b < p.B ? max(__ldg(p.change + b), 0) : 0;
-        long long all, all_asked;
-        const long long end = tokens + bt_scan(add, red, all);
-        const bool fits = len + add <= room && end <= p.max_tokens;
-        const int ask = fits ? bt_blocks(len + add, p.page) - bt_blocks(len, p.page) : 0;
-        const long long upto = asked + bt_scan(ask, red, all_asked);
-        const bool granted = fits && (ask == 0 || upto <= count);
-        long long got;
-        bt_scan(granted ? ask : 0, red, got);
+        const bool row_fits = len + add <= room;
+        bool fits = row_fits;
+        int ask = fits ? bt_blocks(len + add, p.page) - bt_blocks(len, p.page) : 0;
+        Sums all, upto = bt_scan(Sums{add, ask}, red, all);
+        if (tokens + all.a > p.max_tokens) {
+            // some sequence here has tokens behind the slot map's end and asks for nothing: the second sum again
+            fits = row_fits && tokens + upto.a <= p.max_tokens;
+            if (!fits) ask = 0;
+            upto = bt_scan(Sums{add, ask}, red, all);
+        }
+        upto.a += tokens;
+        upto.b += asked;
+        const bool granted = fits && (ask == 0 || upto.b <= count);
+        if (granted && ask) atomicMax(&s_taken, (int)upto.b);          // (who is granted blocks comes before who is not)
         if (b < p.B) {
-            s_end[b] = (int)min(end, 0x7fffffffll);
-            s_off[b] = granted ? (int)(upto - ask) : -1;
+            s_start[b + 1] = (int)min(upto.a, 0x7fffffffll);
+            s_off[b] = (int)min(upto.b - ask, 0x7fffffffll) | (granted ? 0 : BT_REFUSED);
             if (blockIdx.x == 0) {
-                p.starts[b + 1] = s_end[b];
+                p.starts[b + 1] = s_start[b + 1];
                 p.lens_out[b] = (int)(granted ? len + add : len);
             }
         }
-        tokens += all;
-        asked += all_asked;
-        taken += got;
-    }
-    if (blockIdx.x == 0 && tid == 0) {
-        p.starts[0] = 0;
-        *p.count_out = count - (int)taken;
+        tokens += all.a;
+        asked += all.b;
     }
     __syncthreads();
-    // ---- the new entries of the table, a warp per sequence
-    const int lane = tid & 31;
-    const int warps = (int)gridDim.x * (BT_THREADS / 32);
-    for (int b = (int)blockIdx.x * (BT_THREADS / 32) + (tid >> 5); b < p.B; b += warps) {
-        const int off = s_off[b];
-        if (off < 0) continue;
-        const long long len = max(__ldg(p.lens + b), 0);
-        const int add = s_end[b] - (b ? s_end[b - 1] : 0);
-        const int held = bt_blocks(len, p.page), ask = bt_blocks(len + add, p.page) - held;
-        for (int j = lane; j < ask; j += 32) p.table[(size_t)b * p.width + held + j] = __ldg(p.free_blocks + (count - 1 - off - j));
+    const int taken = s_taken;
+    if (blockIdx.x == 0 && tid == 0) {
+        p.starts[0] = 0;
+        *p.count_out = count - taken;
+    }
+    // ---- the new entries of the table
+    const int gtid = (int)blockIdx.x * BT_THREADS + tid, threads = (int)gridDim.x * BT_THREADS;
+    for (int e = gtid; e < taken; e += threads) {
+        const int b = bt_find(s_off, p.B, e);
+        const int held = bt_blocks(max(__ldg(p.lens + b), 0), p.page);
+        p.table[(size_t)b * p.width + held + (e - s_off[b])] = __ldg(p.free_blocks + (count - 1 - e));
     }
     // ---- the slot map, 4 tokens per thread
-    const int last = p.B ? s_end[p.B - 1] : 0;
-    const long long stride = (long long)gridDim.x * BT_THREADS * 4;
-    for (long long t0 = ((long long)blockIdx.x * BT_THREADS + tid) * 4; t0 < p.max_tokens; t0 += stride) {
+    const int last = p.B ? s_start[p.B] : 0;
+    const bool wide = (reinterpret_cast<uintptr_t>(p.slots) & 15u) == 0;
+    for (long long t0 = (long long)gtid * 4; t0 < p.max_tokens; t0 += (long long)threads * 4) {
         int out[4] = {-1, -1, -1, -1};
         int b = -1, end = 0, len = 0, first = 0, off = -1, held = 0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
+            if (t0 + k >= p.max_tokens || t0 + k >= last) break;
             const int t = (int)(t0 + k);
-            if (t0 + k >= p.max_tokens || t >= last) break;
-            if (b < 0 || t >= end) {                   // first sequence whose tokens reach past t
-                int lo = b < 0 ? 0 : b + 1, hi = p.B - 1;
-                if (b >= 0 && s_end[lo] > t) hi = lo;
-                while (lo < hi) {
-                    const int mid = (lo + hi) >> 1;
-                    if (s_end[mid] > t) hi = mid;
-                    else lo = mid + 1;
-                }
-                b = lo;
-                end = s_end[b];
-                first = b ? s_end[b - 1] : 0;
+            if (b < 0 || t >= end) {
+                // the sequence with start <= t < end: the next one that has tokens, most often the next one
+                b = b >= 0 && s_start[b + 2] > t ? b + 1 : bt_find(s_start, p.B + 1, t);
+                first = s_start[b];
+                end = s_start[b + 1];
                 off = s_off[b];
                 len = max(__ldg(p.lens + b), 0);
                 held = bt_blocks(len, p.page);
             }
             if (off < 0) continue;
             const int pos = len + (t - first);         // < width * page
-            const int pg = pos / p.page;
+            const int pg = (int)((unsigned)pos / (unsigned)p.page);
             // entries that this launch writes are taken from where they come from
             const int blk = pg < held ? __ldg(p.table + (size_t)b * p.width + pg)
                                       : __ldg(p.free_blocks + (count - 1 - off - (pg - held)));
             out[k] = blk * p.page + (pos - pg * p.page);
         }
-        if (t0 + 4 <= p.max_tokens && (reinterpret_cast<uintptr_t>(p.slots) & 15u) == 0) {
+        if (wide && t0 + 4 <= p.max_tokens) {
             *reinterpret_cast<int4*>(p.slots + t0) = make_int4(out[0], out[1], out[2], out[3]);
         } else {
 #pragma unroll
@@ -152,41 +168,37 @@ __global__ void __launch_bounds__(BT_THREADS) block_table_extend_kernel(const Bl
 __global__ void __launch_bounds__(BT_THREADS) block_table_trim_kernel(const BlockTableParams p) {
     extern __shared__ int bt_smem[];
     int* s_off = bt_smem;                              // [B] blocks given back before b's
-    __shared__ long long red[BT_THREADS / 32];
+    __shared__ Sums red[BT_THREADS / 32];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x;
     const long long room = (long long)p.width * p.page;
     const int count = min(max(__ldg(p.free_count), 0), p.capacity);
-    auto bounds = [&](int b, int& keep, int& left, int& held) {
-        const int len = (int)min((long long)max(__ldg(p.lens + b), 0), room);
-        keep = min(max(__ldg(p.change + b), 0), len);
-        left = bt_blocks(keep, p.page);
-        held = bt_blocks(len, p.page);
-    };
     long long gone = 0;
     for (int base = 0; base < p.B; base += BT_THREADS) {
         const int b = base + tid;
-        int keep = 0, left = 0, held = 0;
-        if (b < p.B) bounds(b, keep, left, held);
-        long long all;
-        const long long upto = gone + bt_scan(held - left, red, all);
+        int keep = 0, back = 0;
         if (b < p.B) {
-            s_off[b] = (int)min(upto - (held - left), 0x7fffffffll);
+            const int len = (int)min((long long)max(__ldg(p.lens + b), 0), room);
+            keep = min(max(__ldg(p.change + b), 0), len);
+            back = bt_blocks(len, p.page) - bt_blocks(keep, p.page);
+        }
+        Sums all;
+        const Sums upto = bt_scan(Sums{back, 0}, red, all);
+        if (b < p.B) {
+            s_off[b] = (int)min(gone + upto.a - back, 0x7fffffffll);
             if (blockIdx.x == 0) p.lens_out[b] = keep;
         }
-        gone += all;
+        gone += all.a;
     }
-    if (blockIdx.x == 0 && tid == 0) *p.count_out = (int)min(count + gone, (long long)p.capacity);
+    const int pushed = (int)min(gone, (long long)(p.capacity - count));      // (a stack that is full takes no more)
+    if (blockIdx.x == 0 && tid == 0) *p.count_out = count + pushed;
     __syncthreads();
-    const int lane = tid & 31;
-    const int warps = (int)gridDim.x * (BT_THREADS / 32);
-    for (int b = (int)blockIdx.x * (BT_THREADS / 32) + (tid >> 5); b < p.B; b += warps) {
-        int keep, left, held;
-        bounds(b, keep, left, held);
-        const long long at = (long long)count + s_off[b];
-        for (int j = left + lane; j < held; j += 32)
-            if (at + (j - left) < p.capacity) p.free_blocks[at + (j - left)] = __ldg(p.table + (size_t)b * p.width + j);
+    for (int e = (int)blockIdx.x * BT_THREADS + tid; e < pushed; e += (int)gridDim.x * BT_THREADS) {
+        const int b = bt_find(s_off, p.B, e);
+        const int len = (int)min((long long)max(__ldg(p.lens + b), 0), room);
+        const int keep = min(max(__ldg(p.change + b), 0), len);
+        p.free_blocks[count + e] = __ldg(p.table + (size_t)b * p.width + bt_blocks(keep, p.page) + (e - s_off[b]));
     }
 }
 

@@ -60,6 +60,7 @@ struct Q8Params : DecodeParams {
     int4* desc;                // [ncta] unit whose merge starts in this range: (b, unit of b, partials, -)
     int out_dt;                // type of q and out: 0 float32, 1 bfloat16, 2 float16
     int nsplit;                // generic kernel: ranges per unit
+    int device;                // index of the device (host side)
 };
 
 // q and out carry their type at run time: only the first and last step of a unit look at it.

@@ -2,16 +2,22 @@
 // decode_q8_<codes>_<dims>.cu so that they compile side by side.
 #pragma once
 
+#include <atomic>
+
 #include "decode_q8.cuh"
 
 namespace ftk {
 
 template <typename KV, int D, int NBK, bool SPLIT>
 cudaError_t q8_launch_one(const CUtensorMap& mk, const CUtensorMap& mv, const Q8Params& p, cudaStream_t cs) {
-    // a function attribute, not a stream operation: cheap, and legal while the stream is captured
-    cudaError_t e = cudaFuncSetAttribute(decode_q8_kernel<KV, D, NBK, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (Q8Cfg<D, NBK, SPLIT>::SMEM_BYTES));
-    if (e != cudaSuccess) return e;
+    // a function attribute, not a stream operation: legal while the stream is captured. Set once per device.
+    static std::atomic<unsigned long long> done{0};
+    if (!(done.load(std::memory_order_relaxed) >> p.device & 1ull)) {
+        const cudaError_t e = cudaFuncSetAttribute(decode_q8_kernel<KV, D, NBK, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   (Q8Cfg<D, NBK, SPLIT>::SMEM_BYTES));
+        if (e != cudaSuccess) return e;
+        done.fetch_or(1ull << p.device, std::memory_order_relaxed);
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.ncta);
     cfg.blockDim = dim3(Q8_THREADS);

@@ -6,6 +6,7 @@
 #include "../../include/fusedtok_b200.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstring>
 
@@ -31,6 +32,25 @@ __device__ int g_q8_status[64];
 
 int runtime_fail(const char* what, cudaError_t e) {
     return fail(FUSEDTOK_RUNTIME_ERROR, std::string(what) + ": " + cudaGetErrorString(e));
+}
+
+// The current device and its status word (whose address is looked up once per device).
+int status_word(int* device, int** word) {
+    static std::atomic<int*> known[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return runtime_fail("cudaGetDevice", e);
+    if (dev < 0 || dev >= 64) return fail(FUSEDTOK_RUNTIME_ERROR, "device index out of range");
+    int* at = known[dev].load(std::memory_order_relaxed);
+    if (!at) {
+        void* base = nullptr;
+        if ((e = cudaGetSymbolAddress(&base, g_q8_status)) != cudaSuccess) return runtime_fail("status word", e);
+        at = static_cast<int*>(base) + dev;
+        known[dev].store(at, std::memory_order_relaxed);
+    }
+    *device = dev;
+    *word = at;
+    return FUSEDTOK_OK;
 }
 
 // A launch whose kernel begins with griddepcontrol.wait, so that it may be set up while the one before it ends.
@@ -224,12 +244,8 @@ int fusedtok_attention_decode_paged_q8_launch(int dtype, int store, const void* 
     p.ws_acc = reinterpret_cast<float*>(ws + pl.ml_b);
     p.desc = reinterpret_cast<int4*>(ws + pl.ml_b + pl.acc_b);
     p.bound_slots = 2u * (unsigned)pl.ncta;
-    int dev = 0;
-    void* words = nullptr;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaGetSymbolAddress(&words, g_q8_status);
-    if (e != cudaSuccess || dev < 0 || dev >= 64) return runtime_fail("status word", e);
-    p.status = static_cast<int*>(words) + dev;
+    if ((rc = status_word(&p.device, &p.status))) return rc;
+    cudaError_t e = cudaSuccess;
     if (pl.tc) {
         host::EncodeTiledFn encode = nullptr;
         if ((rc = host::encoder(&encode))) return rc;
@@ -284,33 +300,31 @@ int fusedtok_kv_append_paged_q8_launch(int dtype, int store, const void* k_new, 
     p.N = tokens; p.Hkv = kv_heads; p.D = dim; p.page = page;
     p.rows = num_blocks * page;
     const bool wide = es == 2 && dim % 8 == 0 && (news & 15u) == 0 && (pools & 7u) == 0;
-    // a warp where it can hold a block's rows in its registers, else a CTA of four
-    const int vec = wide ? 8 : 4;
-    const int team = (long long)page * dim <= 32ll * AQ_HELD * vec ? 32 : AQ_THREADS;
-    // a token per team while all teams are resident at once, up to a block's worth of tokens beyond
-    const long long heads = 2ll * kv_heads;
-    const long long resident = (long long)sms * (team == 32 ? 20 : 5);
-    p.window = (int)std::max<long long>(1, std::min<long long>({tokens * heads / resident, (long long)page, (long long)team}));
-    p.windows = (tokens + p.window - 1) / p.window;
-    const long long ctas = (p.windows * heads + AQ_THREADS / team - 1) / (AQ_THREADS / team);
+    p.groups = (2 * kv_heads + 3) / 4;
+    // as few tokens per CTA as leave all CTAs resident at once (5 per SM), up to 128
+    const long long work = (long long)tokens * p.groups, room = 5ll * sms;
+    p.window = (int)std::min<long long>((work + room - 1) / room, (long long)AQ_THREADS);
+    const long long ctas = ((tokens + p.window - 1) / p.window) * (long long)p.groups;
     if (ctas > 0x7fffffffll) return fail(FUSEDTOK_INVALID_ARGUMENT, "too many tokens and heads for one launch");
     const dim3 grid((unsigned)ctas);
     cudaStream_t cs = (cudaStream_t)stream;
     const char* what = "8-bit kv append kernel launch";
-#define FTK_TEAM(T, KV, V) \
-    return team == 32 ? launch_pdl(kv_append_q8_kernel<T, KV, V, 32>, grid, dim3(AQ_THREADS), 0, cs, p, what) \
-                      : launch_pdl(kv_append_q8_kernel<T, KV, V, AQ_THREADS>, grid, dim3(AQ_THREADS), 0, cs, p, what)
-#define FTK_GO(T, V)                                  \
-    do {                                              \
-        if (store == 0) FTK_TEAM(T, int8_t, V);       \
-        FTK_TEAM(T, __nv_fp8_e4m3, V);                \
+    // no run is longer than a block
+    const bool lng = (long long)page * dim > (long long)AQ_RING * AQ_BATCH * (wide ? 8 : 4);
+#define FTK_LAUNCH(T, KV, V)                                                                                            \
+    return lng ? launch_pdl(kv_append_q8_kernel<T, KV, V, true>, grid, dim3(AQ_THREADS), 0, cs, p, what)                \
+               : launch_pdl(kv_append_q8_kernel<T, KV, V, false>, grid, dim3(AQ_THREADS), 0, cs, p, what)
+#define FTK_GO(T, V)                                        \
+    do {                                                    \
+        if (store == 0) FTK_LAUNCH(T, int8_t, V);           \
+        FTK_LAUNCH(T, __nv_fp8_e4m3, V);                    \
     } while (0)
     if (dtype == 0) FTK_GO(float, 4);
     if (dtype == 1) { if (wide) FTK_GO(__nv_bfloat16, 8); FTK_GO(__nv_bfloat16, 4); }
     if (wide) FTK_GO(__half, 8);
     FTK_GO(__half, 4);
 #undef FTK_GO
-#undef FTK_TEAM
+#undef FTK_LAUNCH
 }
 
 int fusedtok_block_table_extend_launch(int* table, const int* lens, const int* new_lens, const int* free_blocks,
@@ -325,12 +339,12 @@ int fusedtok_block_table_extend_launch(int* table, const int* lens, const int* n
         return fail(FUSEDTOK_INVALID_ARGUMENT, "null block table operand");
     int sms = 0;
     if ((rc = host::current_sm_count(&sms))) return rc;
-    // 4 slots per thread, 8 sequences' table entries per CTA; every CTA repeats the prefix sums, so no more of them than that
-    const long long want = std::max<long long>(((long long)max_tokens + BT_THREADS * 4 - 1) / (BT_THREADS * 4), (batch + 31) / 32);
+    // 4 slots per thread; every CTA repeats the prefix sums, so no more of them than that and a few for the table
+    const long long want = std::max<long long>(((long long)max_tokens + BT_THREADS * 4 - 1) / (BT_THREADS * 4), (batch + 255) / 256);
     const dim3 grid((unsigned)std::max<long long>(1, std::min<long long>(want, sms)));
-    const size_t smem = (size_t)batch * 8;
+    const size_t smem = (size_t)batch * 8 + 4;
     if (smem > 40000) {
-        const cudaError_t e = cudaFuncSetAttribute(block_table_extend_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BT_MAX_BATCH * 8);
+        const cudaError_t e = cudaFuncSetAttribute(block_table_extend_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BT_MAX_BATCH * 8 + 4);
         if (e != cudaSuccess) return runtime_fail("cudaFuncSetAttribute", e);
     }
     return launch_pdl(block_table_extend_kernel, grid, dim3(BT_THREADS), smem, (cudaStream_t)stream, p, "block table extend launch");
@@ -348,7 +362,9 @@ int fusedtok_block_table_trim_launch(const int* table, const int* lens, const in
         return fail(FUSEDTOK_INVALID_ARGUMENT, "null block table operand");
     int sms = 0;
     if ((rc = host::current_sm_count(&sms))) return rc;
-    const dim3 grid((unsigned)std::max(1, std::min(sms, (batch + 31) / 32)));
+    // an entry per thread if a quarter of all that the table has go back
+    const long long want = ((long long)batch * tbl_width + 4 * BT_THREADS - 1) / (4 * BT_THREADS);
+    const dim3 grid((unsigned)std::max<long long>(1, std::min<long long>(want, sms)));
     return launch_pdl(block_table_trim_kernel, grid, dim3(BT_THREADS), (size_t)batch * 4, (cudaStream_t)stream, p, "block table trim launch");
 }
 

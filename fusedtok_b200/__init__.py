@@ -556,7 +556,10 @@ _CODES = {} if torch is None else {torch.int8: 0, torch.float8_e4m3fn: 1}
 _INT32 = None if torch is None else torch.int32
 _FLOAT32 = None if torch is None else torch.float32
 _q8_workspace = {}       # (device index, shape) -> floats of workspace the launcher asks for
-_device_now = getattr(getattr(torch, "_C", None), "_cuda_getDevice", None)
+# the current device, if its stream can be had without building a Stream object (else no device)
+_device_now = getattr(getattr(torch, "_C", None), "_cuda_getDevice", None) if _raw_stream is not None else None
+if _device_now is None:  # pragma: no cover - other torch builds
+    _device_now = lambda: -1  # noqa: E731
 
 
 def _ready(index, dtype, *tensors):
@@ -570,11 +573,11 @@ def _ready(index, dtype, *tensors):
 
 def _run(index, fn, *args):
     """`fn(*args, stream)` of the C ABI on the current stream of device `index`, its status raised as an exception."""
-    if _raw_stream is None or (_device_now() if _device_now is not None else -1) != index:
+    if _device_now() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
         with torch.cuda.device(index):
             rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
-    else:
-        rc = fn(*args, _raw_stream(index))
     if rc:
         _fusedtok._check(rc)
 
@@ -632,21 +635,24 @@ def attention_decode_paged_q8(q, k_pool, v_pool, kv_scales, block_table, lens=No
         host = _DeviceCall(q=q)
         _q8_cache(host, k_pool, v_pool, kv_scales)
     blocks, hkv, page, dim = _q8_shape(k_pool, v_pool, kv_scales)
-    if len(q.shape) != 3:
-        raise ValueError(f"q: {len(q.shape)}-D tensor where [B, Hq, D] is expected")
-    b, hq, d = q.shape
+    shape = q.shape
+    if len(shape) != 3:
+        raise ValueError(f"q: {len(shape)}-D tensor where [B, Hq, D] is expected")
+    b, hq, d = shape
     if d != dim:
         raise ValueError(f"k_pool: head dim {dim} differs from q's {d}")
-    _gqa_heads(hq, hkv)
+    if hkv < 1 or hq < 1 or hq % hkv:
+        _gqa_heads(hq, hkv)
     if host is not None:
         block_table = host.index("block_table", block_table, (b, None), blocks, False)
         if lens is not None:
             lens = host.index("lens", lens, (b,), block_table.shape[1] * page, True)
-    else:
-        _index_shape("block_table", block_table.shape, (b, None))
-        if lens is not None:
-            _index_shape("lens", lens.shape, (b,))
-    width = block_table.shape[1]
+    elif lens is not None and lens.shape != (b,):
+        _index_shape("lens", lens.shape, (b,))
+    shape = block_table.shape
+    if len(shape) != 2 or shape[0] != b:
+        _index_shape("block_table", shape, (b, None))
+    width = shape[1]
     out = torch.empty_like(q)
     if b:
         code = _STORAGE[q.dtype][1]
@@ -685,17 +691,19 @@ def kv_append_paged_q8(k_pool, v_pool, kv_scales, k_new, v_new, slots):
         call = _DeviceCall(k_new=k_new, v_new=v_new)
         _q8_cache(call, k_pool, v_pool, kv_scales)
     blocks, hkv, page, dim = _q8_shape(k_pool, v_pool, kv_scales)
-    if len(k_new.shape) != 3:
-        raise ValueError(f"k_new: {len(k_new.shape)}-D tensor where [N, Hkv, D] is expected")
-    if v_new.shape != k_new.shape:
-        raise ValueError(f"v_new: shape {tuple(v_new.shape)} differs from k_new's {tuple(k_new.shape)}")
-    n, nh, nd = k_new.shape
+    shape = k_new.shape
+    if len(shape) != 3:
+        raise ValueError(f"k_new: {len(shape)}-D tensor where [N, Hkv, D] is expected")
+    if v_new.shape != shape:
+        raise ValueError(f"v_new: shape {tuple(v_new.shape)} differs from k_new's {tuple(shape)}")
+    n, nh, nd = shape
     if nh != hkv or nd != dim:
         raise ValueError(f"k_new: [Hkv, D] = {(nh, nd)} differs from the cache's {(hkv, dim)}")
     if blocks * page > 0x7fffffff:
         raise ValueError(f"k_pool: {blocks} blocks of {page} rows are more rows than a slot can name")
     if call is None:
-        _index_shape("slots", slots.shape, (n,))
+        if slots.shape != (n,):
+            _index_shape("slots", slots.shape, (n,))
     elif _on_gpu(slots):
         slots = call.index("slots", slots, (n,), blocks * page, False)
     else:
@@ -748,8 +756,10 @@ def _table_operands(page, block_table, lens, change, free_blocks, free_count, ch
             raise TypeError("the block table operators work on CUDA tensors only")
         _DeviceCall(dtypes=(_INT32,), **{"block_table": block_table, "lens": lens, change_name: change,
                                          "free_blocks": free_blocks, "free_count": free_count})
-    _index_shape("block_table", block_table.shape, (None, None))
-    b, width = block_table.shape
+    shape = block_table.shape
+    if len(shape) != 2:
+        _index_shape("block_table", shape, (None, None))
+    b, width = shape
     if lens.shape != (b,):
         _index_shape("lens", lens.shape, (b,))
     if change.shape != (b,):
@@ -758,8 +768,8 @@ def _table_operands(page, block_table, lens, change, free_blocks, free_count, ch
         _index_shape("free_blocks", free_blocks.shape, (None,))
     if free_count.shape != (1,):
         _index_shape("free_count", free_count.shape, (1,))
-    if int(page) != page or page < 1:
-        raise ValueError(f"page {page}: blocks of at least one row are required")
+    if not isinstance(page, int) or page < 1:
+        raise ValueError(f"page {page}: blocks of a whole number of rows, at least one, are required")
     return index, b, width
 
 
@@ -776,15 +786,15 @@ def block_table_extend(block_table, lens, new_lens, free_blocks, free_count, pag
     tensors are contiguous int32 CUDA tensors (at most 8192 sequences), read on the GPU and trusted; free_blocks and
     free_count are not changed - give the returned count to the next call. No counterpart in the reference."""
     index, b, width = _table_operands(page, block_table, lens, new_lens, free_blocks, free_count, "new_lens")
-    if int(max_tokens) != max_tokens or not 0 <= max_tokens <= 0x7fffffff:
+    if not isinstance(max_tokens, int) or not 0 <= max_tokens <= 0x7fffffff:
         raise ValueError(f"max_tokens {max_tokens}: a count of tokens below 2^31 is expected")
-    n = int(max_tokens)
+    n = max_tokens
     made = lens.new_empty(n + 2 * b + 2)                 # one allocation for the four results
     step = BlockTableStep(*made.split_with_sizes([n, b + 1, b, 1]))
     at = made.data_ptr()
     _run(index, _fusedtok._lib.fusedtok_block_table_extend_launch, block_table.data_ptr(), lens.data_ptr(),
          new_lens.data_ptr(), free_blocks.data_ptr(), free_count.data_ptr(), at, at + 4 * n, at + 4 * (n + b + 1),
-         at + 4 * (n + 2 * b + 1), b, width, int(page), free_blocks.shape[0], n)
+         at + 4 * (n + 2 * b + 1), b, width, page, free_blocks.shape[0], n)
     return step
 
 
@@ -797,5 +807,5 @@ def block_table_trim(block_table, lens, keep_lens, free_blocks, free_count, page
     lens_out, left = lens.new_empty(b), lens.new_empty(1)
     _run(index, _fusedtok._lib.fusedtok_block_table_trim_launch, block_table.data_ptr(), lens.data_ptr(),
          keep_lens.data_ptr(), free_blocks.data_ptr(), free_count.data_ptr(), lens_out.data_ptr(), left.data_ptr(), b,
-         width, int(page), free_blocks.shape[0])
+         width, page, free_blocks.shape[0])
     return lens_out, left

@@ -13,7 +13,7 @@
 //  * 8 consumer warps, in 4 groups that take tiles in turn, keep an online softmax over their rows in registers. Nothing
 //    makes them meet: at the end of a segment (the range's part of a unit) a warp leaves its state (m, l, O) in a buffer
 //    and goes on;
-//  * 4 helper warps prepare the query fragments of the next segment and fold the 8 states of the last one. With both done
+//  * 2 helper warps prepare the query fragments of the next segments, 2 fold the 8 states of the last ones. With both done
 //    by the consumers, and barriers between them, every segment cost a CTA about 4 us (12 tiles' worth), and 64 ragged
 //    sequences took 130 us instead of 95.
 //  * Stage layout: a block's (page x D) bytes are contiguous in the pool, so the pool is described to TMA as 128-byte
@@ -46,11 +46,10 @@
 
 namespace ftk {
 
-constexpr int Q8_WPT = 2;                       // consumer warps per tile
-constexpr int Q8_NG = NCW / Q8_WPT;             // groups of warps, taking tiles in turn
-constexpr int Q8_RB = 4 / Q8_WPT;               // 16-row blocks of a tile per warp
-constexpr int Q8_HELPERS = 4;                   // helper warps
-constexpr int Q8_THREADS = (NCW + Q8_HELPERS + Q8_NG) * 32;   // ... and a producer warp per group
+constexpr int Q8_NP = 4;                        // producer warps
+constexpr int Q8_QWARPS = 2, Q8_FWARPS = 2;     // helper warps: query fragments, folds
+constexpr int Q8_HELPERS = Q8_QWARPS + Q8_FWARPS;
+constexpr int Q8_THREADS = (NCW + Q8_HELPERS + Q8_NP) * 32;
 static_assert(Q8_THREADS == 512, "the register split below counts 16 warps");
 constexpr int Q8_MAX_SPLIT = 32;                // generic kernel: most ranges a unit is cut into
 
@@ -126,29 +125,33 @@ template <> struct Codes<__nv_fp8_e4m3> {
     }
 };
 
-template <int D, int NBK, bool SPLIT> struct Q8Cfg {
+template <int D, int NBK, bool SPLIT, int WPT> struct Q8Cfg {
     static_assert(D % 16 == 0 && D >= 64 && D <= 256, "head dim: a multiple of 16 from 64 to 256");
     static constexpr int KV_BYTES = TILE * D;          // a multiple of 1024: the swizzle phase of every stage is the same
     static constexpr int STAGE_BYTES = 2 * KV_BYTES;
     // 128 KB of tiles in flight per SM, as in the 16-bit kernel; a multiple of the number of groups, so that a stage is
     // always consumed by the same group, which then sees every phase of its barrier in order
-    static constexpr int NS = (131072 / STAGE_BYTES) / Q8_NG * Q8_NG;
-    static_assert(NS >= Q8_NG, "ring shorter than the groups");
+    static constexpr int NG = NCW / WPT;               // groups of consumer warps, taking tiles in turn
+    static constexpr int RB = 4 / WPT;                 // 16-row blocks of a tile per warp
+    static constexpr int NS = (131072 / STAGE_BYTES) / NG * NG;
+    static_assert(NS >= NG && NS % Q8_NP == 0, "ring shorter than the groups");
     static constexpr int HEADS = NBK * (SPLIT ? 4 : 8);
     static constexpr int ACC_STRIDE = D + 4;
     static constexpr int STATE_BYTES = NCW * HEADS * ACC_STRIDE * 4;             // the warps' O of one segment
-    static constexpr int NF = STATE_BYTES <= 34816 ? 2 : 1;                      // segments whose states may wait to be folded
+    // segments whose states may wait to be folded: as many as fit beside the ring (sequences of a tile or two keep several
+    // segments in flight; 256 of 60 - 200 rows: 44 us with two)
+    static constexpr int NF = STATE_BYTES <= 17408 ? 4 : STATE_BYTES <= 34816 ? 2 : 1;
+    static constexpr int NQ = NF == 4 ? 4 : 2;         // segments whose query fragments may be ready
     static constexpr int Q_BYTES = NBK * (D / 16) * 32 * 8;                      // query fragments of a segment
     // The CTA is launched with 128 registers per thread; the 2 consumer warpgroups take more, the 2 others give up as many.
     static constexpr int REGS_CONSUMER = NBK * D <= 128 ? 152 : 168, REGS_OTHER = 256 - REGS_CONSUMER;
     static constexpr int OFF_STATE = NS * STAGE_BYTES;
     static constexpr int OFF_ML = OFF_STATE + NF * STATE_BYTES;                  // [NF][NCW][HEADS] (m, l)
-    static constexpr int OFF_Q = OFF_ML + NF * NCW * HEADS * 8;                  // [2] fragments
-    static constexpr int OFF_KF = OFF_Q + 2 * Q_BYTES;                           // [2][16] score factors
-    static constexpr int OFF_W = OFF_KF + 2 * 16 * 4;                            // [HEADS][NCW] weights of the fold, [HEADS] l
-    static constexpr int OFF_SCALE = OFF_W + 16 * (NCW + 1) * 4;                 // [NS][4] (K, V) scales of the stage's blocks
-    static constexpr int OFF_BAR = OFF_SCALE + NS * 4 * 8;                       // full[NS], empty[NS], q full / empty [2], state full / empty [2]
-    static constexpr int OFF_SCHED = OFF_BAR + (2 * NS + 8) * 8;
+    static constexpr int OFF_Q = OFF_ML + NF * NCW * HEADS * 8;                  // [NQ] fragments
+    static constexpr int OFF_KF = OFF_Q + NQ * Q_BYTES;                          // [NQ][16] score factors
+    static constexpr int OFF_SCALE = OFF_KF + NQ * 16 * 4;                       // [NS][4] (K, V) scales of the stage's blocks
+    static constexpr int OFF_BAR = OFF_SCALE + NS * 4 * 8;                       // full[NS], empty[NS], q full / empty [NQ], state full / empty [4]
+    static constexpr int OFF_SCHED = OFF_BAR + (2 * NS + 2 * NQ + 8) * 8;
     static constexpr int OFF_ABORT = OFF_SCHED + (int)sizeof(SchedShared);
     static constexpr int OFF_PREFIX = (OFF_ABORT + 16 + 15) & ~15;
     static constexpr int OFF_ZPRE = OFF_PREFIX + (SCHED_MAX_B + 1) * 4;
@@ -181,18 +184,18 @@ __device__ __forceinline__ void row_exponent(float x, float& f, float& g) {
 
 // ---- the kernel ----------------------------------------------------------------
 // KV: code type. NBK: 8-column blocks of the MMA. SPLIT: two columns per query head (see above).
-template <typename KV, int D, int NBK, bool SPLIT>
+template <typename KV, int D, int NBK, bool SPLIT, int WPT>
 __global__ void __launch_bounds__(Q8_THREADS, 1)
 decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Q8Params p) {
-    using Cfg = Q8Cfg<D, NBK, SPLIT>;
+    using Cfg = Q8Cfg<D, NBK, SPLIT, WPT>;
     extern __shared__ __align__(1024) uint8_t smem[];
     SchedShared* sh = reinterpret_cast<SchedShared*>(smem + Cfg::OFF_SCHED);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Cfg::OFF_ABORT);
     const uint32_t smem_base = smem_u32(smem);
     const uint32_t bar_full = smem_base + Cfg::OFF_BAR;
     const uint32_t bar_empty = bar_full + Cfg::NS * 8;
-    const uint32_t bar_q_full = bar_empty + Cfg::NS * 8, bar_q_empty = bar_q_full + 16;
-    const uint32_t bar_state_full = bar_q_empty + 16, bar_state_empty = bar_state_full + 16;
+    const uint32_t bar_q_full = bar_empty + Cfg::NS * 8, bar_q_empty = bar_q_full + Cfg::NQ * 8;
+    const uint32_t bar_state_full = bar_q_empty + Cfg::NQ * 8, bar_state_empty = bar_state_full + 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int cta = (int)blockIdx.x;
 
@@ -204,13 +207,15 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         }
         for (int s = 0; s < Cfg::NS; ++s) {
             mbar_init(bar_full + s * 8, 33);           // the announced bytes, and each producer lane's scales
-            mbar_init(bar_empty + s * 8, Q8_WPT);
+            mbar_init(bar_empty + s * 8, WPT);
         }
-        for (int s = 0; s < 2; ++s) {
-            mbar_init(bar_q_full + s * 8, Q8_HELPERS);
+        for (int s = 0; s < Cfg::NQ; ++s) {
+            mbar_init(bar_q_full + s * 8, Q8_QWARPS);
             mbar_init(bar_q_empty + s * 8, NCW);
+        }
+        for (int s = 0; s < Cfg::NF; ++s) {
             mbar_init(bar_state_full + s * 8, NCW);
-            mbar_init(bar_state_empty + s * 8, Q8_HELPERS);
+            mbar_init(bar_state_empty + s * 8, Q8_FWARPS);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_k) : "memory");
@@ -226,7 +231,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     if (!p.lens) {
         total = (long long)p.B * tiles_of(p.T) * upb;
         pl = make_plan(total, p.ncta, 0, 0);
-        if (total > 0) plan_enable_cost(pl, (long long)p.B * tiles_of(p.T), p.B, upb, nullptr, nullptr, tiles_of(p.T), 1, 1);
+        if (total > 0) plan_enable_cost(pl, (long long)p.B * tiles_of(p.T), p.B, upb, nullptr, nullptr, tiles_of(p.T), 1, 3);
         asm volatile("griddepcontrol.wait;" ::: "memory");
     } else {
         asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -236,7 +241,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         prefix = table;
         zprefix = ztable;
         pl = make_plan(total, p.ncta, 0, 0);
-        if (total > 0) plan_enable_cost(pl, prefix[p.B], zprefix[p.B], upb, prefix, zprefix, 0, 1, 1);
+        if (total > 0) plan_enable_cost(pl, prefix[p.B], zprefix[p.B], upb, prefix, zprefix, 0, 1, 3);
     }
     if (*abort_flag) {
         if (threadIdx.x == 0) p.desc[cta] = make_int4(0, 0, 0, 0);
@@ -251,46 +256,41 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 
     constexpr int KSTEPS = D / 16;
     constexpr int HB = SPLIT ? 4 : 8;              // query heads per column block
-    constexpr int HEADS = Cfg::HEADS;
+    constexpr int HEADS = Cfg::HEADS, RB = Cfg::RB;
 
     if (warp >= NCW + Q8_HELPERS) {
         // ===================== producer warps =====================
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_OTHER));
-        // One per group of consumer warps: it issues that group's tiles (every Q8_NG-th of the range). A single one would
-        // have to issue a 16 KB tile of 2 KB blocks every 350 ns, and falls behind (measured: 94 us instead of 47).
-        const int cg = warp - NCW - Q8_HELPERS;
+        // Every Q8_NP-th tile of the range. A single producer would have to issue a 16 KB tile of 2 KB blocks every 350 ns,
+        // and falls behind (measured: 94 us for 32 x 4096 rows instead of 57). A tile's table entries are fetched while the
+        // tile before it goes out.
+        const int pw = warp - NCW - Q8_HELPERS;
         const uint64_t pol = policy_evict_first();
         const int page_shift = __ffs(p.page) - 1;
-        const int per_tile = 1 << (6 - p.box_shift);                        // blocks (or parts of one) a tile has
-        // Table entries, one per lane: lane (k, j) holds block j of this warp's k-th next tile, as far as the unit goes,
-        // and another set the entries of the tiles behind those, on their way
-        const int lane_row = (lane >> (6 - p.box_shift)) * (Q8_NG * TILE) + ((lane & (per_tile - 1)) << p.box_shift);
-        const int reach = 32 >> (6 - p.box_shift);                          // tiles a set covers
-        int at = reach, tbl_val = 0, tbl_next = 0, unit_b = -1, unit_ub = -1;
-        int issued = 0, s = cg;
+        int issued = 0, s = pw;
         uint32_t ph = 0;
         bool gave_up = false;
-        for (int i = 0; i < cg && w.g < w.end; ++i) walker_advance(p, w);
+        auto blocks_of = [&](const Walker& t) {                             // blocks (or parts of one) tile t has rows in
+            return p.page <= TILE ? (min(TILE, t.len - t.ti * TILE) + p.page - 1) >> p.box_shift : 1;
+        };
+        auto entry = [&](const Walker& t) {                                 // lane j: the j-th of them
+            return lane < blocks_of(t) ? __ldg(p.table + (size_t)t.b * p.tbl_width + ((t.ti * TILE + (lane << p.box_shift)) >> page_shift)) : 0;
+        };
+        for (int i = 0; i < pw && w.g < w.end; ++i) walker_advance(p, w);
+        int blk = w.g < w.end ? entry(w) : 0;
         while (w.g < w.end) {
-            const int kv = w.ub / p.NCH;
-            const int t0 = w.ti * TILE;
-            auto entry = [&](int row) { return row < w.len ? __ldg(p.table + (size_t)w.b * p.tbl_width + (row >> page_shift)) : 0; };
-            if (w.b != unit_b || w.ub != unit_ub) {
-                unit_b = w.b;
-                unit_ub = w.ub;
-                at = 0;
-                tbl_val = entry(t0 + lane_row);
-                tbl_next = entry(t0 + reach * (Q8_NG * TILE) + lane_row);
-            } else if (at == reach) {
-                at = 0;
-                tbl_val = tbl_next;
-                tbl_next = entry(t0 + reach * (Q8_NG * TILE) + lane_row);
+            Walker next = w;
+            if (w.ti + Q8_NP < w.nt) {
+                next.g += Q8_NP;
+                next.ti += Q8_NP;
+            } else {
+                for (int i = 0; i < Q8_NP && next.g < next.end; ++i) walker_advance(p, next);
             }
-            const int npg = p.page <= TILE ? (min(TILE, w.len - t0) + p.page - 1) >> p.box_shift : 1;
-            int blk = __shfl_sync(0xffffffffu, tbl_val, (at * per_tile + lane) & 31);
-            ++at;
-            if (lane < npg && !(blk >= 0 && blk < p.blocks)) blk = 0;      // (device table values are trusted: address only)
-            const long long unit_row = ((long long)blk * p.Hkv + kv) * p.page + (p.page <= TILE ? 0 : t0 & (p.page - 1));
+            const int next_blk = next.g < next.end ? entry(next) : 0;
+            const int kv = w.ub / p.NCH;
+            const int npg = blocks_of(w);
+            if (!(blk >= 0 && blk < p.blocks)) blk = 0;                     // (device table values are trusted: address only)
+            const long long unit_row = ((long long)blk * p.Hkv + kv) * p.page + (p.page <= TILE ? 0 : (w.ti * TILE) & (p.page - 1));
             const int line = (int)(unit_row * D >> 7);
             const uint32_t bytes = (uint32_t)(npg << p.box_shift) * (uint32_t)(2 * D);
             if (!mbar_wait(bar_empty + s * 8, ph ^ 1u, abort_flag, p.status, ST_WAIT_EMPTY_TIMEOUT)) {
@@ -308,24 +308,20 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
             }
             cp_async_arrive(fb);
             ++issued;
-            if (w.ti + Q8_NG < w.nt) {
-                w.g += Q8_NG;
-                w.ti += Q8_NG;
-            } else {
-                for (int i = 0; i < Q8_NG && w.g < w.end; ++i) walker_advance(p, w);
-            }
-            s += Q8_NG;
+            w = next;
+            blk = next_blk;
+            s += Q8_NP;
             if (s >= Cfg::NS) { s -= Cfg::NS; ph ^= 1u; }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         if (gave_up || *abort_flag) {
             // do not leave the CTA while its own copies may still be landing: wait (bounded) for the last phase of every
             // stage this warp issued
-            constexpr int OWN = Cfg::NS / Q8_NG;
+            constexpr int OWN = Cfg::NS / Q8_NP;
             const int first = issued > OWN ? issued - OWN : 0;
             for (int i = first; i < issued; ++i) {
                 const unsigned long long b0 = global_ns();
-                while (!mbar_try_wait(bar_full + (cg + (i % OWN) * Q8_NG) * 8, (uint32_t)((i / OWN) & 1))) {
+                while (!mbar_try_wait(bar_full + (pw + (i % OWN) * Q8_NP) * 8, (uint32_t)((i / OWN) & 1))) {
                     if (global_ns() - b0 > WAIT_LIMIT_NS) {
                         atomicCAS(p.status, ST_OK, ST_DRAIN_TIMEOUT);
                         break;
@@ -339,41 +335,51 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     if (warp >= NCW) {
         // ===================== helper warps =====================
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_OTHER));
-        const int hw = warp - NCW, tid = threadIdx.x - NCW * 32;
-        float* s_w = reinterpret_cast<float*>(smem + Cfg::OFF_W);
-        auto helpers = [] { asm volatile("bar.sync 2, %0;" ::"n"(Q8_HELPERS * 32) : "memory"); };
-        // The query rows of a unit as B fragments, each row scaled by a power of two into the range of a half. A warp
-        // takes every fourth head; a lane the 4 elements that make a fragment register pair.
-        auto prepare_q = [&](int k, const Walker& u) {
-            const int buf = k & 1;
-            mbar_wait(bar_q_empty + buf * 8, (uint32_t)((k >> 1) & 1) ^ 1u, abort_flag, p.status, ST_WAIT_RANGE_TIMEOUT);
-            const int kv = u.ub / p.NCH, ch = u.ub % p.NCH;
-            const int gvalid = min(p.GC, p.G - ch * p.GC);
-            const size_t row0 = ((size_t)u.b * p.Hq + kv * p.G + ch * p.GC) * D;
-            uint2* frag = reinterpret_cast<uint2*>(smem + Cfg::OFF_Q + buf * Cfg::Q_BYTES);
-            float* kf = reinterpret_cast<float*>(smem + Cfg::OFF_KF) + buf * 16;
-            constexpr int PER = (HEADS + Q8_HELPERS - 1) / Q8_HELPERS, LR = (D / 4 + 31) / 32;
+        // tiles of the segment that begins at t, and the step to the next segment
+        auto seg_tiles = [](const Walker& t) { return (int)min(t.end - t.g, (long long)(t.nt - t.ti)); };
+        auto to_next = [&](Walker& t) {
+            const int n = seg_tiles(t);
+            t.g += n - 1;
+            t.ti += n - 1;
+            walker_advance(p, t);
+        };
+        if (warp < NCW + Q8_QWARPS) {
+            // ---- The query rows of each segment's unit as B fragments, each row scaled by a power of two into the range of
+            // a half. A warp takes every other head; a lane the 4 elements that make a fragment register pair. The rows
+            // are requested one segment before they are worked on.
+            const int hw = warp - NCW;
+            constexpr int PER = (HEADS + Q8_QWARPS - 1) / Q8_QWARPS, LR = (D / 4 + 31) / 32;
             float4 x[PER][LR];
+            auto request = [&]() {
+                const int kv = w.ub / p.NCH, ch = w.ub - kv * p.NCH;
+                const int gvalid = min(p.GC, p.G - ch * p.GC);
+                const size_t row0 = ((size_t)w.b * p.Hq + kv * p.G + ch * p.GC) * D;
 #pragma unroll
-            for (int i = 0; i < PER; ++i)
+                for (int i = 0; i < PER; ++i)
 #pragma unroll
-                for (int r = 0; r < LR; ++r) {
-                    const int g = hw + i * Q8_HELPERS, c = lane + 32 * r;
-                    x[i][r] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (g < gvalid && c < D / 4) x[i][r] = load4_any(p.q, row0 + (size_t)g * D + c * 4, p.out_dt);
-                }
+                    for (int r = 0; r < LR; ++r) {
+                        const int g = hw + i * Q8_QWARPS, c = lane + 32 * r;
+                        x[i][r] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (g < gvalid && c < D / 4) x[i][r] = load4_any(p.q, row0 + (size_t)g * D + c * 4, p.out_dt);
+                    }
+            };
+            if (w.g < w.end) request();
+            for (int k = 0; w.g < w.end; ++k) {
+                const int buf = k % Cfg::NQ;
+                mbar_wait(bar_q_empty + buf * 8, (uint32_t)((k / Cfg::NQ) & 1) ^ 1u, abort_flag, p.status, ST_WAIT_RANGE_TIMEOUT);
+                uint2* frag = reinterpret_cast<uint2*>(smem + Cfg::OFF_Q + buf * Cfg::Q_BYTES);
+                float* kf = reinterpret_cast<float*>(smem + Cfg::OFF_KF) + buf * 16;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const int g = hw + i * Q8_HELPERS;
-                uint32_t top = 0;                       // as bits: NaN and infinity are the largest
+                for (int i = 0; i < PER; ++i) {
+                    const int g = hw + i * Q8_QWARPS;
+                    uint32_t top = 0;                       // as bits: NaN and infinity are the largest
 #pragma unroll
-                for (int r = 0; r < LR; ++r)
-                    top = max(max(top, max(__float_as_uint(x[i][r].x) & 0x7fffffffu, __float_as_uint(x[i][r].y) & 0x7fffffffu)),
-                              max(__float_as_uint(x[i][r].z) & 0x7fffffffu, __float_as_uint(x[i][r].w) & 0x7fffffffu));
-                top = __reduce_max_sync(0xffffffffu, top);
-                float fx, gx;
-                row_exponent(__uint_as_float(top), fx, gx);
-                if (g < HEADS) {
+                    for (int r = 0; r < LR; ++r)
+                        top = max(max(top, max(__float_as_uint(x[i][r].x) & 0x7fffffffu, __float_as_uint(x[i][r].y) & 0x7fffffffu)),
+                                  max(__float_as_uint(x[i][r].z) & 0x7fffffffu, __float_as_uint(x[i][r].w) & 0x7fffffffu));
+                    top = __reduce_max_sync(0xffffffffu, top);
+                    float fx, gx;
+                    row_exponent(__uint_as_float(top), fx, gx);
 #pragma unroll
                     for (int r = 0; r < LR; ++r) {
                         const int c = lane + 32 * r;
@@ -392,83 +398,74 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
                     }
                     if (lane == 0) kf[g] = gx * p.scale * LOG2E;
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_q_full + buf * 8);
+                to_next(w);
+                if (w.g < w.end) request();
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar_q_full + buf * 8);
-        };
+            return;
+        }
+        // ---- The consumers' states of each segment, folded into the output or into a partial.
+        const int tid = threadIdx.x - (NCW + Q8_QWARPS) * 32;
         int4 merge = make_int4(0, 0, 0, 0);           // the unit that begins in this range and ends in a later one
         if (w.g >= w.end) {
             // nothing here: an empty partial, which a merge that spans this range passes over
-            for (int i = tid; i < p.GC; i += Q8_HELPERS * 32)
+            for (int i = tid; i < p.GC; i += Q8_FWARPS * 32)
                 *reinterpret_cast<float2*>(p.ws_ml + ((size_t)2 * cta * p.GC + i) * 2) = make_float2(-INFINITY, 0.0f);
-        } else {
-            prepare_q(0, w);
         }
         for (int k = 0; w.g < w.end; ++k) {
-            const long long left = w.end - w.g;
-            const int n = (int)(left < (long long)(w.nt - w.ti) ? left : (long long)(w.nt - w.ti));
+            const int n = seg_tiles(w);
             const bool begins = w.ti == 0, ends = w.ti + n == w.nt, whole = begins && ends;
-            const Walker u = w;
-            w.g += n - 1;
-            w.ti += n - 1;
-            walker_advance(p, w);
-            if (w.g < w.end) prepare_q(k + 1, w);
-            const int kv = u.ub / p.NCH, ch = u.ub % p.NCH;
+            const int kv = w.ub / p.NCH, ch = w.ub - kv * p.NCH;
             const int gvalid = min(p.GC, p.G - ch * p.GC);
-            const size_t out0 = ((size_t)u.b * p.Hq + kv * p.G + ch * p.GC) * D;
+            const size_t out0 = ((size_t)w.b * p.Hq + kv * p.G + ch * p.GC) * D;
             const size_t slot = (size_t)2 * cta + (begins ? 1 : 0);
+            if (begins && !ends) {
+                int last;
+                if (pl.ctot) last = cost_owner(pl, cost_of_unit(pl, w.b, w.ub, w.nt) + (long long)pl.ka * (w.nt - 1));
+                else last = range_of(pl, w.g + w.nt - 1);              // w stands on the unit's first tile
+                merge = make_int4(w.b, w.ub, last - cta + 1, 0);
+            }
+            to_next(w);
             const int buf = k % Cfg::NF;
             const float* s_acc = reinterpret_cast<const float*>(smem + Cfg::OFF_STATE + buf * Cfg::STATE_BYTES);
             const float2* s_ml = reinterpret_cast<const float2*>(smem + Cfg::OFF_ML) + buf * NCW * HEADS;
             mbar_wait(bar_state_full + buf * 8, (uint32_t)((k / Cfg::NF) & 1), abort_flag, p.status, ST_WAIT_FULL_TIMEOUT);
-            // weights of the warps' states; -1: a warp that had no tile of this segment and left no O
-            if (tid < HEADS) {
-                float m = -INFINITY, l = 0.0f;
+            for (int it = tid; it < gvalid * (D / 4); it += Q8_FWARPS * 32) {
+                const int g = it / (D / 4), d = (it % (D / 4)) * 4;
+                // Every thread works the weights of its head out for itself: 8 exponentials, and no barrier. A warp that had
+                // no tile of this segment (l == 0) left no O: what is read in its place is not used.
                 float2 ml[NCW];
+                float4 v[NCW];
+                float m = -INFINITY, l = 0.0f;
 #pragma unroll
                 for (int ww = 0; ww < NCW; ++ww) {
-                    ml[ww] = s_ml[ww * HEADS + tid];
+                    ml[ww] = s_ml[ww * HEADS + g];
+                    v[ww] = *reinterpret_cast<const float4*>(s_acc + ((size_t)ww * HEADS + g) * Cfg::ACC_STRIDE + d);
                     m = fmaxf(m, ml[ww].x);
                 }
                 const float safe = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-                for (int ww = 0; ww < NCW; ++ww) {
-                    const float f = ex2(ml[ww].x - safe);
-                    l += ml[ww].y != 0.0f ? ml[ww].y * f : 0.0f;
-                    s_w[tid * NCW + ww] = ml[ww].y != 0.0f ? f : -1.0f;
-                }
-                if (whole) l = l != 0.0f ? 1.0f / l : 0.0f;
-                else if (tid < gvalid && FTK_SLOT_OK(p, slot, 0))
-                    *reinterpret_cast<float2*>(p.ws_ml + (slot * p.GC + tid) * 2) = make_float2(m, l);
-                s_w[16 * NCW + tid] = l;
-            }
-            helpers();
-            for (int it = tid; it < gvalid * (D / 4); it += Q8_HELPERS * 32) {
-                const int g = it / (D / 4), d = (it % (D / 4)) * 4;
                 float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (int ww = 0; ww < NCW; ++ww) {
-                    const float f = s_w[g * NCW + ww];
-                    float4 v = *reinterpret_cast<const float4*>(s_acc + ((size_t)ww * HEADS + g) * Cfg::ACC_STRIDE + d);
-                    if (f == -1.0f) v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    a.x = fmaf(v.x, f, a.x); a.y = fmaf(v.y, f, a.y); a.z = fmaf(v.z, f, a.z); a.w = fmaf(v.w, f, a.w);
+                    const bool some = ml[ww].y != 0.0f;
+                    const float f = ex2(ml[ww].x - safe);
+                    l = fmaf(ml[ww].y, f, l);
+                    a.x = fmaf(some ? v[ww].x : 0.0f, f, a.x);
+                    a.y = fmaf(some ? v[ww].y : 0.0f, f, a.y);
+                    a.z = fmaf(some ? v[ww].z : 0.0f, f, a.z);
+                    a.w = fmaf(some ? v[ww].w : 0.0f, f, a.w);
                 }
                 if (whole) {
-                    const float inv = s_w[16 * NCW + g];
+                    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
                     store4_any(p.out, out0 + (size_t)g * D + d, p.out_dt, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
                 } else if (FTK_SLOT_OK(p, slot, 0)) {
                     *reinterpret_cast<float4*>(p.ws_acc + (slot * p.GC + g) * D + d) = a;
+                    if (d == 0) *reinterpret_cast<float2*>(p.ws_ml + (slot * p.GC + g) * 2) = make_float2(m, l);
                 }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_state_empty + buf * 8);
-            helpers();                                // the weights are free again
-            if (begins && !ends) {
-                int last;
-                if (pl.ctot) last = cost_owner(pl, cost_of_unit(pl, u.b, u.ub, u.nt) + (long long)pl.ka * (u.nt - 1));
-                else last = range_of(pl, u.g + u.nt - 1);              // u stands on the unit's first tile
-                merge = make_int4(u.b, u.ub, last - cta + 1, 0);
-            }
         }
         if (tid == 0) p.desc[cta] = merge;
         return;
@@ -476,7 +473,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 
     // ======================= consumer warps =======================
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_CONSUMER));
-    const int cg = warp / Q8_WPT, wr = warp % Q8_WPT;
+    const int cg = warp / WPT, wr = warp % WPT;
     const int quad = lane >> 2, qi = lane & 3;
     const float neg_inf = -INFINITY;
 
@@ -491,7 +488,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     // Byte offset of chunk 2 i + csel of row r inside a tile, swizzled. `csel` and the row are the lane's.
     const int lrow = ((lane >> 3) & 1) * 8 + (lane & 7), csel = lane >> 4;
     auto chunk_off = [&](int j, int i) -> uint32_t {
-        const uint32_t lin = (uint32_t)((wr * Q8_RB + j) * 16 + lrow) * (uint32_t)D + (uint32_t)(2 * i + csel) * 16u;
+        const uint32_t lin = (uint32_t)((wr * RB + j) * 16 + lrow) * (uint32_t)D + (uint32_t)(2 * i + csel) * 16u;
         return lin ^ (((lin >> 7) & 7u) << 4);
     };
 
@@ -503,23 +500,23 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         const uint32_t st_k = smem_base + s * Cfg::STAGE_BYTES;
         const uint32_t st_v = st_k + Cfg::KV_BYTES;
         const float2* sc = reinterpret_cast<const float2*>(smem + Cfg::OFF_SCALE) + s * 4;
-        float2 ks[Q8_RB];
+        float2 ks[RB];
 #pragma unroll
-        for (int j = 0; j < Q8_RB; ++j) {
-            const int r0 = (wr * Q8_RB + j) * 16;
+        for (int j = 0; j < RB; ++j) {
+            const int r0 = (wr * RB + j) * 16;
             ks[j] = sc[r0 >> p.box_shift];
             // a block of the tile that holds no valid row was not copied, nor were its scales
             if (RAGGED && r0 >= rows_valid) ks[j] = make_float2(0.0f, 0.0f);
         }
         constexpr int PF = 2;
-        constexpr int N = Q8_RB * NLD;
+        constexpr int N = RB * NLD;
         uint32_t f[PF][4];
         // ---- S^T = K Q^T
-        float sa[NBK][Q8_RB][4];
+        float sa[NBK][RB][4];
 #pragma unroll
         for (int nbk = 0; nbk < NBK; ++nbk)
 #pragma unroll
-            for (int j = 0; j < Q8_RB; ++j) sa[nbk][j][0] = sa[nbk][j][1] = sa[nbk][j][2] = sa[nbk][j][3] = 0.0f;
+            for (int j = 0; j < RB; ++j) sa[nbk][j][0] = sa[nbk][j][1] = sa[nbk][j][2] = sa[nbk][j][3] = 0.0f;
 #pragma unroll
         for (int n = 0; n < PF; ++n) ldsm_x4(st_k + chunk_off(n / NLD, n % NLD), f[n][0], f[n][1], f[n][2], f[n][3]);
 #pragma unroll
@@ -544,26 +541,26 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         for (int n = 0; n < PF; ++n) ldsm_x4_t(st_v + chunk_off(n / NLD, n % NLD), f[n][0], f[n][1], f[n][2], f[n][3]);
         // ---- online softmax, in units of log2
         if (e0 < 0) e0 = (int)min(max((__float_as_uint(ks[0].y) >> 23) & 255u, 64u), 190u);
-        float de[Q8_RB], ge[Q8_RB], ce[Q8_RB];    // per block: exponent of vs less e0, 2^-that, and what is left of vs
+        float de[RB], ge[RB], ce[RB];    // per block: exponent of vs less e0, 2^-that, and what is left of vs
 #pragma unroll
-        for (int j = 0; j < Q8_RB; ++j) {
+        for (int j = 0; j < RB; ++j) {
             const int d = min(max((int)((__float_as_uint(ks[j].y) >> 23) & 255u) - e0, -60), 60);
             de[j] = (float)d;
             ge[j] = __uint_as_float((uint32_t)(127 - d) << 23);
             ce[j] = ks[j].y * __uint_as_float((uint32_t)(254 - (e0 + d)) << 23);
         }
-        uint32_t pb[NBK][Q8_RB][2];
+        uint32_t pb[NBK][RB][2];
 #pragma unroll
         for (int nbk = 0; nbk < NBK; ++nbk) {
-            float pw[HPT][Q8_RB][2];
+            float pw[HPT][RB][2];
 #pragma unroll
             for (int e = 0; e < HPT; ++e) {
-                float v[Q8_RB][2];
+                float v[RB][2];
                 float mx = neg_inf;
 #pragma unroll
-                for (int j = 0; j < Q8_RB; ++j) {
+                for (int j = 0; j < RB; ++j) {
                     const float fac = kf[nbk][e] * ks[j].x;
-                    const int r_lo = (wr * Q8_RB + j) * 16 + quad;
+                    const int r_lo = (wr * RB + j) * 16 + quad;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         v[j][h] = fmaf(SPLIT ? sa[nbk][j][2 * h] + sa[nbk][j][2 * h + 1] : sa[nbk][j][2 * h + e], fac, de[j]);
@@ -579,7 +576,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
                 const float m_safe = m_new == neg_inf ? 0.0f : m_new;
                 float sum = 0.0f;
 #pragma unroll
-                for (int j = 0; j < Q8_RB; ++j)
+                for (int j = 0; j < RB; ++j)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const float w8 = ex2(v[j][h] - m_safe);
@@ -604,7 +601,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
                 l_run[nbk][e] += sum;
             }
 #pragma unroll
-            for (int j = 0; j < Q8_RB; ++j)
+            for (int j = 0; j < RB; ++j)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     if constexpr (SPLIT) {
@@ -622,7 +619,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
             uint32_t (&r)[4] = f[n % PF];
             if constexpr (RAGGED) {
                 // rows at and past the end may hold anything, NaN codes included: a zero weight times them has to be zero
-                const int t = (wr * Q8_RB + j) * 16 + qi * 2;
+                const int t = (wr * RB + j) * 16 + qi * 2;
                 const uint32_t lo = (t < rows_valid ? 0x0000ffffu : 0u) | (t + 1 < rows_valid ? 0xffff0000u : 0u);
                 const uint32_t hi = (t + 8 < rows_valid ? 0x0000ffffu : 0u) | (t + 9 < rows_valid ? 0xffff0000u : 0u);
                 r[0] &= lo; r[1] &= hi; r[2] &= lo; r[3] &= hi;
@@ -650,8 +647,8 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         // ---- the segment's query fragments
         e0 = -1;
         {
-            const int buf = k & 1;
-            mbar_wait(bar_q_full + buf * 8, (uint32_t)((k >> 1) & 1), abort_flag, p.status, ST_WAIT_RANGE_TIMEOUT);
+            const int buf = k % Cfg::NQ;
+            mbar_wait(bar_q_full + buf * 8, (uint32_t)((k / Cfg::NQ) & 1), abort_flag, p.status, ST_WAIT_RANGE_TIMEOUT);
             if (mine) {
                 const uint2* frag = reinterpret_cast<const uint2*>(smem + Cfg::OFF_Q + buf * Cfg::Q_BYTES) + lane;
                 const float* s_kf = reinterpret_cast<const float*>(smem + Cfg::OFF_KF) + buf * 16;
@@ -681,16 +678,16 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
             for (int mt = 0; mt < KSTEPS; ++mt) acc[nbk][mt][0] = acc[nbk][mt][1] = acc[nbk][mt][2] = acc[nbk][mt][3] = 0.0f;
         }
         // ---- this group's tiles of the segment
-        for (; own < i0 + n; own += Q8_NG) {
+        for (; own < i0 + n; own += Cfg::NG) {
             const bool ok = mbar_wait(bar_full + s * 8, ph, abort_flag, p.status, ST_WAIT_FULL_TIMEOUT);
             const int rows_valid = w.len - (w.ti + (own - i0)) * TILE;      // >= 1
             if (ok) {
                 if (rows_valid >= TILE) process(std::false_type{}, TILE);
-                else if (wr * (Q8_RB * 16) < rows_valid) process(std::true_type{}, rows_valid);
+                else if (wr * (RB * 16) < rows_valid) process(std::true_type{}, rows_valid);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_empty + s * 8);
-            s += Q8_NG;
+            s += Cfg::NG;
             if (s >= Cfg::NS) { s -= Cfg::NS; ph ^= 1u; }
         }
         i0 += n;

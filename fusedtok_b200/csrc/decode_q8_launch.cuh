@@ -10,25 +10,29 @@ namespace ftk {
 
 template <typename KV, int D, int NBK, bool SPLIT>
 cudaError_t q8_launch_one(const CUtensorMap& mk, const CUtensorMap& mv, const Q8Params& p, cudaStream_t cs) {
+    // warps per 64-row tile: with two a warp has 32 rows to overlap work over (one: 53 us instead of 49 for 32 x 4096 rows
+    // of 128, too many registers; four: 50, and 94 instead of 90 for ragged ones); wide heads have work enough in 16 rows (256:
+    // 51 us instead of 57)
+    constexpr int WPT = D >= 192 ? 4 : 2;
     // a function attribute, not a stream operation: legal while the stream is captured. Set once per device.
     static std::atomic<unsigned long long> done{0};
     if (!(done.load(std::memory_order_relaxed) >> p.device & 1ull)) {
-        const cudaError_t e = cudaFuncSetAttribute(decode_q8_kernel<KV, D, NBK, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   (Q8Cfg<D, NBK, SPLIT>::SMEM_BYTES));
+        const cudaError_t e = cudaFuncSetAttribute(decode_q8_kernel<KV, D, NBK, SPLIT, WPT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   (Q8Cfg<D, NBK, SPLIT, WPT>::SMEM_BYTES));
         if (e != cudaSuccess) return e;
         done.fetch_or(1ull << p.device, std::memory_order_relaxed);
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.ncta);
     cfg.blockDim = dim3(Q8_THREADS);
-    cfg.dynamicSmemBytes = (Q8Cfg<D, NBK, SPLIT>::SMEM_BYTES);
+    cfg.dynamicSmemBytes = (Q8Cfg<D, NBK, SPLIT, WPT>::SMEM_BYTES);
     cfg.stream = cs;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, decode_q8_kernel<KV, D, NBK, SPLIT>, mk, mv, p);
+    return cudaLaunchKernelEx(&cfg, decode_q8_kernel<KV, D, NBK, SPLIT, WPT>, mk, mv, p);
 }
 
 template <typename KV, int D>

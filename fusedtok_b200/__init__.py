@@ -598,6 +598,13 @@ def _q8_cache(call, k_pool, v_pool, kv_scales):
         raise TypeError(f"v_pool: dtype {v_pool.dtype} differs from k_pool's {k_pool.dtype}")
 
 
+def _whole(label, values):
+    """Refuse a CUDA index tensor that does not hold whole numbers (host values are checked where they are read)."""
+    if _on_gpu(values) and (values.is_floating_point() or values.is_complex() or values.dtype is torch.bool):
+        raise TypeError(f"{label}: integer values expected, found {values.dtype}")
+    return values
+
+
 def _q8_shape(k_pool, v_pool, kv_scales):
     """(Nb, Hkv, P, D) of an 8-bit cache whose shapes agree."""
     shape = k_pool.shape
@@ -644,9 +651,9 @@ def attention_decode_paged_q8(q, k_pool, v_pool, kv_scales, block_table, lens=No
     if hkv < 1 or hq < 1 or hq % hkv:
         _gqa_heads(hq, hkv)
     if host is not None:
-        block_table = host.index("block_table", block_table, (b, None), blocks, False)
+        block_table = host.index("block_table", _whole("block_table", block_table), (b, None), blocks, False)
         if lens is not None:
-            lens = host.index("lens", lens, (b,), block_table.shape[1] * page, True)
+            lens = host.index("lens", _whole("lens", lens), (b,), block_table.shape[1] * page, True)
     elif lens is not None and lens.shape != (b,):
         _index_shape("lens", lens.shape, (b,))
     shape = block_table.shape
@@ -659,6 +666,8 @@ def attention_decode_paged_q8(q, k_pool, v_pool, kv_scales, block_table, lens=No
         key = (index, code, b, hq, hkv, page, width, d)
         floats = _q8_workspace.get(key)
         if floats is None:
+            if len(_q8_workspace) >= 4096:
+                _q8_workspace.clear()
             with torch.cuda.device(index):
                 floats = _q8_workspace[key] = (_fusedtok.attention_decode_paged_q8_workspace(*key[1:]) + 3) // 4
         scratch = kv_scales.new_empty(floats)
@@ -679,8 +688,8 @@ def kv_append_paged_q8(k_pool, v_pool, kv_scales, k_new, v_new, slots):
     (int8) or 448 (e4m3): ``old = scale if o > 0 else 0; new = max(old, max|x| / M)``; rows before ``o`` get the codes
     ``round(code * old / new)``, the new ones ``round(x / new)`` (to the nearest code, ties to even); rows behind stay.
     A value that is not finite makes the block's scale NaN. CUDA tensors only; host slots are checked (``< Nb * P``,
-    and the rule above), a CUDA tensor is trusted (slots outside the pool are passed over). No counterpart in the
-    reference."""
+    and the rule above), a CUDA tensor is trusted (slots outside the pool are passed over). The pools must not overlap. No
+    counterpart in the reference."""
     index = k_pool.get_device() if isinstance(k_pool, _Tensor) else -1
     call = None
     if not (isinstance(k_new, _Tensor) and k_new.dtype in _STORAGE and _ready(index, k_new.dtype, k_new, v_new)
@@ -705,7 +714,9 @@ def kv_append_paged_q8(k_pool, v_pool, kv_scales, k_new, v_new, slots):
         if slots.shape != (n,):
             _index_shape("slots", slots.shape, (n,))
     elif _on_gpu(slots):
-        slots = call.index("slots", slots, (n,), blocks * page, False)
+        if slots.dtype is torch.int64:               # (a slot that int32 cannot hold is outside the pool: keep it there)
+            slots = slots.clamp(-1, 0x7fffffff)
+        slots = call.index("slots", _whole("slots", slots), (n,), blocks * page, False)
     else:
         slots = torch.from_numpy(_host_slots(slots, n, blocks, page)).to(call.device)
     if n:
@@ -768,7 +779,7 @@ def _table_operands(page, block_table, lens, change, free_blocks, free_count, ch
         _index_shape("free_blocks", free_blocks.shape, (None,))
     if free_count.shape != (1,):
         _index_shape("free_count", free_count.shape, (1,))
-    if not isinstance(page, int) or page < 1:
+    if not isinstance(page, (int, np.integer)) or page < 1:
         raise ValueError(f"page {page}: blocks of a whole number of rows, at least one, are required")
     return index, b, width
 
@@ -786,15 +797,15 @@ def block_table_extend(block_table, lens, new_lens, free_blocks, free_count, pag
     tensors are contiguous int32 CUDA tensors (at most 8192 sequences), read on the GPU and trusted; free_blocks and
     free_count are not changed - give the returned count to the next call. No counterpart in the reference."""
     index, b, width = _table_operands(page, block_table, lens, new_lens, free_blocks, free_count, "new_lens")
-    if not isinstance(max_tokens, int) or not 0 <= max_tokens <= 0x7fffffff:
+    if not isinstance(max_tokens, (int, np.integer)) or not 0 <= max_tokens <= 0x7fffffff:
         raise ValueError(f"max_tokens {max_tokens}: a count of tokens below 2^31 is expected")
-    n = max_tokens
+    n = int(max_tokens)
     made = lens.new_empty(n + 2 * b + 2)                 # one allocation for the four results
     step = BlockTableStep(*made.split_with_sizes([n, b + 1, b, 1]))
     at = made.data_ptr()
     _run(index, _fusedtok._lib.fusedtok_block_table_extend_launch, block_table.data_ptr(), lens.data_ptr(),
          new_lens.data_ptr(), free_blocks.data_ptr(), free_count.data_ptr(), at, at + 4 * n, at + 4 * (n + b + 1),
-         at + 4 * (n + 2 * b + 1), b, width, page, free_blocks.shape[0], n)
+         at + 4 * (n + 2 * b + 1), b, width, int(page), free_blocks.shape[0], n)
     return step
 
 
@@ -807,5 +818,5 @@ def block_table_trim(block_table, lens, keep_lens, free_blocks, free_count, page
     lens_out, left = lens.new_empty(b), lens.new_empty(1)
     _run(index, _fusedtok._lib.fusedtok_block_table_trim_launch, block_table.data_ptr(), lens.data_ptr(),
          keep_lens.data_ptr(), free_blocks.data_ptr(), free_count.data_ptr(), lens_out.data_ptr(), left.data_ptr(), b,
-         width, page, free_blocks.shape[0])
+         width, int(page), free_blocks.shape[0])
     return lens_out, left

@@ -289,7 +289,9 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
             const int next_blk = next.g < next.end ? entry(next) : 0;
             const int kv = w.ub / p.NCH;
             const int npg = blocks_of(w);
-            if (!(blk >= 0 && blk < p.blocks)) blk = 0;                     // (device table values are trusted: address only)
+            // (device table values are trusted; an entry outside the pool only has to stay an address, and is reported by the
+            // self-checking build)
+            if (!FTK_ROW_OK(p, ((long long)blk * p.Hkv + kv) * p.page) || !(blk >= 0 && blk < p.blocks)) blk = 0;
             const long long unit_row = ((long long)blk * p.Hkv + kv) * p.page + (p.page <= TILE ? 0 : (w.ti * TILE) & (p.page - 1));
             const int line = (int)(unit_row * D >> 7);
             const uint32_t bytes = (uint32_t)(npg << p.box_shift) * (uint32_t)(2 * D);
@@ -776,7 +778,7 @@ decode_q8_generic_kernel(const Q8Params p) {
         for (int r = 0; r < R; ++r) {
             const int t = min(t0 + r, end - 1);
             int blk = __ldg(p.table + (size_t)b * p.tbl_width + t / p.page);
-            if (!(blk >= 0 && blk < p.blocks)) blk = 0;
+            if (!FTK_ROW_OK(p, ((long long)blk * p.Hkv + kv) * p.page) || !(blk >= 0 && blk < p.blocks)) blk = 0;
             sc[r] = __ldg(p.scales + (size_t)blk * p.Hkv + kv);
             const size_t row = ((size_t)blk * p.Hkv + kv) * p.page + t % p.page;
 #pragma unroll

@@ -244,6 +244,7 @@ int fusedtok_attention_decode_paged_q8_launch(int dtype, int store, const void* 
     p.ws_acc = reinterpret_cast<float*>(ws + pl.ml_b);
     p.desc = reinterpret_cast<int4*>(ws + pl.ml_b + pl.acc_b);
     p.bound_slots = 2u * (unsigned)pl.ncta;
+    p.bound_rows = (unsigned long long)num_blocks * kv_heads * page;
     if ((rc = status_word(&p.device, &p.status))) return rc;
     cudaError_t e = cudaSuccess;
     if (pl.tc) {
@@ -290,6 +291,9 @@ int fusedtok_kv_append_paged_q8_launch(int dtype, int store, const void* k_new, 
     const uintptr_t pools = reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool);
     if ((news & (4 * es - 1)) || (pools & 3u) || (reinterpret_cast<uintptr_t>(kv_scales) & 3u))
         return fail(FUSEDTOK_INVALID_ARGUMENT, "new rows must be aligned to 4 elements, pools and scales to 4 bytes");
+    const uintptr_t ka = reinterpret_cast<uintptr_t>(k_pool), va = reinterpret_cast<uintptr_t>(v_pool);
+    if ((ka < va ? va - ka : ka - va) < (unsigned long long)num_blocks * kv_heads * page * dim)
+        return fail(FUSEDTOK_INVALID_ARGUMENT, "the K and V pools must not overlap");
     int sms = 0;
     const int rc = host::current_sm_count(&sms);
     if (rc) return rc;

@@ -299,7 +299,8 @@ int fusedtok_attention_decode_launch_noalloc(int dtype, const void* q, const voi
  *
  * attention_decode_paged_q8: fusedtok_attention_decode_paged_launch over such a
  * cache (same shapes, head mapping, scale and zero rows; any GQA group; a block
- * table entry outside [0, num_blocks) is read as block 0). Accumulation in float32.
+ * table entry outside [0, num_blocks) is read as block 0). Accumulation in float32;
+ * the V scales of one sequence's blocks may differ by a factor of up to 2^60.
  * `workspace`: 16-byte aligned device memory of at least
  * fusedtok_attention_decode_paged_q8_workspace(...) bytes that the call may
  * overwrite and no other work may touch until it is done (its contents before
@@ -319,7 +320,7 @@ int fusedtok_attention_decode_launch_noalloc(int dtype, const void* q, const voi
  * Rows behind the run keep their codes (they stand for nothing until they are
  * appended). new == 0 gives codes 0; a NaN or infinity among the run's values
  * makes the scale NaN, and the block reads as NaN until it is begun again at
- * offset 0. D % 4 == 0, D <= 512, Nb * P < 2^31. */
+ * offset 0. D % 4 == 0, D <= 512, Nb * P < 2^31; the two pools must not overlap. */
 long long fusedtok_attention_decode_paged_q8_workspace(int dtype, int batch, int q_heads, int kv_heads, int page,
                                                        int tbl_width, int dim);
 int fusedtok_attention_decode_paged_q8_launch(int dtype, int store, const void* q, const void* k_pool,

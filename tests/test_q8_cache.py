@@ -98,10 +98,11 @@ def test_launchers_refuse_before_touching_the_gpu():
         with pytest.raises(ValueError):
             lib.attention_decode_paged_q8_launch(**{**good, **change})
     lib.attention_decode_paged_q8_launch(**{**good, "batch": 0})
-    good = dict(dtype=1, store=0, k_new=64, v_new=64, slots=64, k_pool=64, v_pool=64, kv_scales=64, tokens=1, hkv=2, dim=64,
+    good = dict(dtype=1, store=0, k_new=64, v_new=64, slots=64, k_pool=64, v_pool=1 << 20, kv_scales=64, tokens=1, hkv=2, dim=64,
                 page=16, num_blocks=8)
     for change in (dict(dtype=-1), dict(store=5), dict(tokens=-1), dict(hkv=0), dict(dim=2), dict(dim=1024), dict(page=0),
-                   dict(num_blocks=1 << 28), dict(k_new=0), dict(slots=0), dict(kv_scales=0), dict(k_new=68), dict(v_pool=65)):
+                   dict(num_blocks=1 << 28), dict(k_new=0), dict(slots=0), dict(kv_scales=0), dict(k_new=68), dict(v_pool=65),
+                   dict(v_pool=64), dict(v_pool=64 + 8 * 2 * 16 * 64 - 4)):
         with pytest.raises(ValueError):
             lib.kv_append_paged_q8_launch(**{**good, **change})
     lib.kv_append_paged_q8_launch(**{**good, "tokens": 0})
@@ -295,7 +296,8 @@ def test_decode_refusals():
     run = ft().attention_decode_paged_q8
     run(q, kp, vp, s, t)
     for bad in ((q.double(), kp, vp, s, t), (q, kp.float(), vp, s, t), (q, kp, vp.view(torch.float8_e4m3fn), s, t),
-                (q, kp, vp, s.half(), t), (q, kp.cpu(), vp, s, t), (q, kp, vp, s, t, [0.5, 1.0])):
+                (q, kp, vp, s.half(), t), (q, kp.cpu(), vp, s, t), (q, kp, vp, s, t, [0.5, 1.0]),
+                (q, kp, vp, s, t, torch.ones(2, device="cuda")), (q, kp, vp, s, t.bool())):
         with pytest.raises(TypeError):
             run(*bad)
     for bad in ((q[:, :3], kp, vp, s, t), (q[..., :60].contiguous(), kp, vp, s, t), (q, kp, vp[:-1], s, t), (q, kp, vp, s[:-1], t),
@@ -510,17 +512,19 @@ def test_append_unaligned(name):
 @pytest.mark.gpu
 def test_append_refusals():
     kp = torch.zeros((4, 2, 16, 64), dtype=torch.int8, device="cuda")
+    vp = kp.clone()
     s, x = torch.zeros((4, 2, 2), device="cuda"), torch.zeros((3, 2, 64), device="cuda")
     run = ft().kv_append_paged_q8
     run(kp, kp.clone(), s, x, x, [0, 1, 2])
-    for bad in ((kp, kp, s, x.cpu(), x, [0, 1, 2]), (kp, kp, s, x, x.half(), [0, 1, 2]), (kp, kp, s, x.double(), x.double(), [0, 1, 2]),
-                (kp.short(), kp.short(), s, x, x, [0, 1, 2]), (kp, kp, s, x, x, [0.0, 1.0, 2.0])):
+    for bad in ((kp, vp, s, x.cpu(), x, [0, 1, 2]), (kp, vp, s, x, x.half(), [0, 1, 2]), (kp, vp, s, x.double(), x.double(), [0, 1, 2]),
+                (kp.short(), vp.short(), s, x, x, [0, 1, 2]), (kp, vp, s, x, x, [0.0, 1.0, 2.0]),
+                (kp, vp, s, x, x, torch.zeros(3, device="cuda"))):
         with pytest.raises(TypeError):
             run(*bad)
-    for bad in ((kp, kp, s, x, x[:2], [0, 1, 2]), (kp, kp, s, x[:, :1].contiguous(), x[:, :1].contiguous(), [0, 1, 2]),
-                (kp, kp, s, x, x, [0, 1]), (kp, kp, s, x, x, [0, 1, 64]), (kp, kp, s, x, x, [0, 1, 1]),
-                (kp, kp, s[:2], x, x, [0, 1, 2]), (kp, kp[..., :32].contiguous(), s, x, x, [0, 1, 2]),
-                (kp, kp, s, x.transpose(0, 1), x, [0, 1, 2])):
+    for bad in ((kp, kp, s, x, x, [0, 1, 2]), (kp, vp, s, x, x[:2], [0, 1, 2]), (kp, vp, s, x[:, :1].contiguous(), x[:, :1].contiguous(), [0, 1, 2]),
+                (kp, vp, s, x, x, [0, 1]), (kp, vp, s, x, x, [0, 1, 64]), (kp, vp, s, x, x, [0, 1, 1]),
+                (kp, vp, s[:2], x, x, [0, 1, 2]), (kp, vp[..., :32].contiguous(), s, x, x, [0, 1, 2]),
+                (kp, vp, s, x.transpose(0, 1), x, [0, 1, 2])):
         with pytest.raises(ValueError):
             run(*bad)
 
@@ -739,3 +743,144 @@ def test_same_bits_every_call():
     first = ft().attention_decode_paged_q8(*args)
     for _ in range(20):
         assert torch.equal(first, ft().attention_decode_paged_q8(*args))
+
+
+@pytest.mark.gpu
+def test_index_tensors_of_other_types():
+    """int64 tables, lengths and slots (PyTorch's default) give what int32 ones give; a slot beyond 32 bits is passed over,
+    not wrapped into the pool; host arrays and strided index tensors too."""
+    rng = np.random.default_rng(13)
+    lens = [100, 37]
+    k, v, scales, table = make_cache(rng, lens, 2, 64, 16, "int8")
+    q = rounded(rng.standard_normal((2, 4, 64)), "bf16").cuda()
+    a = (pool(k, "int8"), pool(v, "int8"), on_gpu(scales))
+    want = ft().attention_decode_paged_q8(q, *a, on_gpu(table), on_gpu(np.array(lens, np.int32)))
+    wide = on_gpu(np.repeat(table, 2, axis=1).astype(np.int64))[:, ::2]
+    for t in (on_gpu(table.astype(np.int64)), wide, table, torch.from_numpy(table)):
+        for n in (on_gpu(np.array(lens)), lens, np.array(lens, np.int16)):
+            assert torch.equal(want, ft().attention_decode_paged_q8(q, *a, t, n))
+    x = rounded(rng.standard_normal((4, 2, 64)), "f16").cuda()
+    slots = np.array([2 ** 32 + 3, table[0, 1] * 16 + 2, -2 ** 33, 2 ** 31 - 1])
+    kq, vq, s = (t.clone() for t in a)
+    ft().kv_append_paged_q8(kq, vq, s, x, x, on_gpu(slots))
+    ref.append(k, scales, 0, x.double().cpu().numpy(), [-1, slots[1], -1, -1], 16, "int8")
+    assert (codes_of(kq) == k).all() and (s.cpu().numpy()[..., 0] == scales[..., 0]).all()
+
+
+@pytest.mark.gpu
+def test_every_code():
+    """All 256 codes are read as what they stand for (int8 -128 among them, which an append never writes)."""
+    for store in STORES:
+        codes = np.arange(256, dtype=np.uint8)
+        codes = codes[np.isfinite(ref.decode_codes(codes, store))]
+        for dim, page in ((64, 16), (128, 16), (20, 7)):
+            n = -(-len(codes) // dim) * dim
+            rows = np.resize(codes, n).reshape(-1, dim)
+            for row in rows:
+                pools = np.zeros((1, 1, page, dim), np.uint8)
+                pools[0, 0, 0] = row
+                scales = np.array([[[0.0, 0.37]]], np.float32)
+                out = ft().attention_decode_paged_q8(torch.ones((1, 1, dim), device="cuda"), pool(pools, store), pool(pools, store),
+                                                     on_gpu(scales), [[0]], [1])
+                want = ref.decode_codes(row, store) * np.float64(np.float32(0.37))
+                # one weight of exactly 1 in two halves, codes exact: the scale's product and its factors, a few half steps
+                assert (np.abs(out.double().cpu().numpy()[0, 0] - want) <= np.abs(want) * 2.0 ** -21).all()
+
+
+_SELF_CHECKING = """
+import sys, numpy as np, torch
+sys.path.insert(0, %r); sys.path.insert(0, %r)
+import test_q8_cache as t
+from fusedtok_b200 import _fusedtok
+for shape in t.SHAPES:
+    b, hq, hkv, d, page, lens = shape
+    rng = np.random.default_rng(1)
+    k, v, scales, table = t.make_cache(rng, lens, hkv, d, page, "e4m3")
+    q = t.rounded(rng.standard_normal((b, hq, d)), "bf16")
+    t.check_decode(q, k, v, scales, table, lens, "e4m3", "bf16")
+    assert _fusedtok.attention_device_status() == 0, shape
+    table[0, 0] = len(k) + 3 if hq %% 2 else -1       # outside the pool: reported, read as block 0
+    t.ft().attention_decode_paged_q8(q.cuda(), t.pool(k, "e4m3"), t.pool(v, "e4m3"), t.on_gpu(scales), t.on_gpu(table),
+                                     t.on_gpu(np.array(lens, np.int32)))
+    assert _fusedtok.attention_device_status() == (8 if lens[0] else 0), shape
+    assert _fusedtok.attention_device_status() == 0
+print("self-checked")
+"""
+
+
+@pytest.mark.gpu
+def test_self_checking_build():
+    """The build that compares every computed row and slot with what the launch owns (see test_bounds_build_gpu.py)."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    variant = os.path.join(os.path.dirname(here), "fusedtok_b200", "libfusedtok_b200_bounds.so")
+    if not os.path.exists(variant):
+        pytest.skip("self-checking variant of the library not built")
+    done = subprocess.run([sys.executable, "-c", _SELF_CHECKING % (os.path.dirname(here), here)], capture_output=True, text=True,
+                          timeout=600, env=dict(os.environ, FUSEDTOK_B200_LIB=variant))
+    assert done.returncode == 0 and "self-checked" in done.stdout, done.stdout + done.stderr
+
+
+_FIRST_CALLS_CAPTURED = """
+import sys, numpy as np, torch
+sys.path.insert(0, %r); sys.path.insert(0, %r)
+import test_q8_cache as t
+state, alone = t._step_state(5, %d, %d), t._step_state(5, %d, %d)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = t._decode_step(state)                   # the first calls of the library in this process
+got = []
+for _ in range(3):
+    g.replay()
+    got.append(out.clone())
+torch.cuda.synchronize()
+for x in got:
+    assert torch.equal(x, t._decode_step(alone))
+for key in ("k", "v", "s", "table", "lens", "count"):
+    assert torch.equal(state[key].view(torch.uint8), alone[key].view(torch.uint8)), key
+print("captured first")
+"""
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page,dim", [(16, 128), (12, 64)])
+def test_first_calls_of_a_process_are_captured(page, dim):
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = _FIRST_CALLS_CAPTURED % (os.path.dirname(here), here, page, dim, page, dim)
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured first" in done.stdout, done.stdout + done.stderr
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_and_threads():
+    """Calls that overlap on different streams, issued from different threads, share nothing."""
+    import threading
+    rng = np.random.default_rng(14)
+    cases = []
+    for i in range(3):
+        lens = [4000 - 700 * i, 17, 900]
+        k, v, scales, table = make_cache(rng, lens, 2, 128, 16, "e4m3")
+        cases.append((rounded(rng.standard_normal((3, 8, 128)), "bf16").cuda(), pool(k, "e4m3"), pool(v, "e4m3"), on_gpu(scales),
+                      on_gpu(table), on_gpu(np.array(lens, np.int32))))
+    want = [ft().attention_decode_paged_q8(*c) for c in cases]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            outs = [ft().attention_decode_paged_q8(*cases[i]) for _ in range(50)]
+        stream.synchronize()
+        bad.extend(i for o in outs if not torch.equal(o, want[i]))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad

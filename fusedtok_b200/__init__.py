@@ -553,38 +553,30 @@ def rope_kv_append_paged(q, k_pool, v_pool, block_table, k_new, v_new, lens, *, 
 
 # code type of the pools -> store code of the C ABI
 _CODES = {} if torch is None else {torch.int8: 0, torch.float8_e4m3fn: 1}
-_INT32 = None if torch is None else torch.int32
-_FLOAT32 = None if torch is None else torch.float32
-_q8_workspace = {}       # (device index, shape) -> floats of workspace the launcher asks for
-# the current device, if its stream can be had without building a Stream object (else no device)
-_device_now = getattr(getattr(torch, "_C", None), "_cuda_getDevice", None) if _raw_stream is not None else None
-if _device_now is None:  # pragma: no cover - other torch builds
-    _device_now = lambda: -1  # noqa: E731
 
 
-def _ready(index, dtype, *tensors):
-    """True if all are contiguous tensors of `dtype` on CUDA device `index`: the quick look that the calls of a decode
-    loop pass. Where it fails, the careful checks find out why."""
-    for t in tensors:
-        if not (isinstance(t, _Tensor) and t.dtype is dtype and t.get_device() == index and t.is_contiguous()):
-            return False
-    return index >= 0
+def _native(name):
+    """`name` of the module that makes the plain calls - operands that need no conversion - from tensors to the C ABI in
+    one step (csrc/tensor_calls.cpp), bound to the loaded library. It returns None for every other call, which then takes
+    the careful way below; so does every call where the module has not been built."""
+    return getattr(_tensors, name) if _tensors is not None else lambda *operands: None
 
 
-def _run(index, fn, *args):
-    """`fn(*args, stream)` of the C ABI on the current stream of device `index`, its status raised as an exception."""
-    if _device_now() == index:
-        rc = fn(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
-    if rc:
-        _fusedtok._check(rc)
+def _whole(label, values):
+    """Refuse a CUDA index tensor that does not hold whole numbers (host values are checked where they are read)."""
+    if _on_gpu(values) and (values.is_floating_point() or values.is_complex() or values.dtype is torch.bool):
+        raise TypeError(f"{label}: integer values expected, found {values.dtype}")
+    return values
 
 
-def _q8_cache(call, k_pool, v_pool, kv_scales):
-    """Raise what is wrong with the cache operands of a call (the activations are checked: `call`)."""
-    for name, t, allowed in (("k_pool", k_pool, _CODES), ("v_pool", v_pool, _CODES), ("kv_scales", kv_scales, (_FLOAT32,))):
+def _q8_operands(lead, k_pool, v_pool, kv_scales, **rest):
+    """Checks common to the operators on an 8-bit paged cache: activations `rest` of one storage type, pools of one
+    code type, float32 scales, everything contiguous on one device. Returns (call, store, Nb, Hkv, P, D)."""
+    if not _on_gpu(lead):
+        raise TypeError("the operators on an 8-bit cache work on CUDA tensors only")
+    call = _DeviceCall(**rest)
+    for name, t, allowed in (("k_pool", k_pool, _CODES), ("v_pool", v_pool, _CODES),
+                             ("kv_scales", kv_scales, (torch.float32,))):
         if not _on_gpu(t):
             raise TypeError(f"{name}: a CUDA tensor is required")
         if t.dtype not in allowed:
@@ -596,28 +588,16 @@ def _q8_cache(call, k_pool, v_pool, kv_scales):
             raise ValueError(f"{name}: a contiguous tensor is required")
     if v_pool.dtype is not k_pool.dtype:
         raise TypeError(f"v_pool: dtype {v_pool.dtype} differs from k_pool's {k_pool.dtype}")
-
-
-def _whole(label, values):
-    """Refuse a CUDA index tensor that does not hold whole numbers (host values are checked where they are read)."""
-    if _on_gpu(values) and (values.is_floating_point() or values.is_complex() or values.dtype is torch.bool):
-        raise TypeError(f"{label}: integer values expected, found {values.dtype}")
-    return values
-
-
-def _q8_shape(k_pool, v_pool, kv_scales):
-    """(Nb, Hkv, P, D) of an 8-bit cache whose shapes agree."""
-    shape = k_pool.shape
-    if len(shape) != 4:
-        raise ValueError(f"k_pool: {len(shape)}-D tensor where [Nb, Hkv, P, D] is expected")
-    if v_pool.shape != shape:
-        raise ValueError(f"v_pool: shape {tuple(v_pool.shape)} differs from k_pool's {tuple(shape)}")
-    blocks, hkv, page, dim = shape
+    if k_pool.ndim != 4:
+        raise ValueError(f"k_pool: {k_pool.ndim}-D tensor where [Nb, Hkv, P, D] is expected")
+    if v_pool.shape != k_pool.shape:
+        raise ValueError(f"v_pool: shape {tuple(v_pool.shape)} differs from k_pool's {tuple(k_pool.shape)}")
+    blocks, hkv, page, dim = k_pool.shape
     if kv_scales.shape != (blocks, hkv, 2):
         raise ValueError(f"kv_scales: shape {tuple(kv_scales.shape)} where {(blocks, hkv, 2)} follows from the pools")
     if page < 1:
         raise ValueError("k_pool: blocks of at least one row are required")
-    return blocks, hkv, page, dim
+    return call, _CODES[k_pool.dtype], blocks, hkv, page, dim
 
 
 def attention_decode_paged_q8(q, k_pool, v_pool, kv_scales, block_table, lens=None):
@@ -631,50 +611,27 @@ def attention_decode_paged_q8(q, k_pool, v_pool, kv_scales, block_table, lens=No
     ``attention_decode_paged``. Any GQA group. The V scales of one sequence's blocks may differ by a factor of up to
     2^60. CUDA tensors only; host table and lens values are checked, CUDA tensors trusted. The scratch of a call comes
     from torch's allocator, so calls on different streams do not share any. No counterpart in the reference."""
-    index = q.get_device() if isinstance(q, _Tensor) else -1
-    given = (block_table,) if lens is None else (block_table, lens)
-    host = None
-    if not (q.dtype in _STORAGE and _ready(index, q.dtype, q) and getattr(k_pool, "dtype", None) in _CODES
-            and _ready(index, k_pool.dtype, k_pool, v_pool) and _ready(index, _FLOAT32, kv_scales)
-            and _ready(index, _INT32, *given)) if index >= 0 else True:
-        if not _on_gpu(q):
-            raise TypeError("the operators on an 8-bit cache work on CUDA tensors only")
-        host = _DeviceCall(q=q)
-        _q8_cache(host, k_pool, v_pool, kv_scales)
-    blocks, hkv, page, dim = _q8_shape(k_pool, v_pool, kv_scales)
-    shape = q.shape
-    if len(shape) != 3:
-        raise ValueError(f"q: {len(shape)}-D tensor where [B, Hq, D] is expected")
-    b, hq, d = shape
+    out = _decode_q8_native(q, k_pool, v_pool, kv_scales, block_table, lens)
+    if out is not None:
+        return out
+    call, store, blocks, hkv, page, dim = _q8_operands(q, k_pool, v_pool, kv_scales, q=q)
+    b, hq, d = call.dims("q", "B Hq D")
     if d != dim:
         raise ValueError(f"k_pool: head dim {dim} differs from q's {d}")
-    if hkv < 1 or hq < 1 or hq % hkv:
-        _gqa_heads(hq, hkv)
-    if host is not None:
-        block_table = host.index("block_table", _whole("block_table", block_table), (b, None), blocks, False)
-        if lens is not None:
-            lens = host.index("lens", _whole("lens", lens), (b,), block_table.shape[1] * page, True)
-    elif lens is not None and lens.shape != (b,):
-        _index_shape("lens", lens.shape, (b,))
-    shape = block_table.shape
-    if len(shape) != 2 or shape[0] != b:
-        _index_shape("block_table", shape, (b, None))
-    width = shape[1]
-    out = torch.empty_like(q)
+    _gqa_heads(hq, hkv)
+    table = call.index("block_table", _whole("block_table", block_table), (b, None), blocks, False)
+    width = table.shape[1]
+    if lens is not None:
+        lens = call.index("lens", _whole("lens", lens), (b,), width * page, True)
+    out = call.new((b, hq, d))
     if b:
-        code = _STORAGE[q.dtype][1]
-        key = (index, code, b, hq, hkv, page, width, d)
-        floats = _q8_workspace.get(key)
-        if floats is None:
-            if len(_q8_workspace) >= 4096:
-                _q8_workspace.clear()
-            with torch.cuda.device(index):
-                floats = _q8_workspace[key] = (_fusedtok.attention_decode_paged_q8_workspace(*key[1:]) + 3) // 4
-        scratch = kv_scales.new_empty(floats)
-        _run(index, _fusedtok._lib.fusedtok_attention_decode_paged_q8_launch, code, _CODES[k_pool.dtype], q.data_ptr(),
-             k_pool.data_ptr(), v_pool.data_ptr(), kv_scales.data_ptr(), block_table.data_ptr(),
-             None if lens is None else lens.data_ptr(), out.data_ptr(), scratch.data_ptr(), 4 * floats, b, hq, hkv, page,
-             width, blocks, d)
+        shape = (b, hq, hkv, page, width)
+        with torch.cuda.device(call.device):
+            need = _fusedtok.attention_decode_paged_q8_workspace(call.code, *shape, d)
+        scratch = torch.empty(need, dtype=torch.uint8, device=call.device)
+        call.launch(_fusedtok.attention_decode_paged_q8_launch, call.code, store, q.data_ptr(), k_pool.data_ptr(),
+                    v_pool.data_ptr(), kv_scales.data_ptr(), table.data_ptr(), None if lens is None else lens.data_ptr(),
+                    out.data_ptr(), scratch.data_ptr(), need, *shape, blocks, d)
     return out
 
 
@@ -688,41 +645,27 @@ def kv_append_paged_q8(k_pool, v_pool, kv_scales, k_new, v_new, slots):
     (int8) or 448 (e4m3): ``old = scale if o > 0 else 0; new = max(old, max|x| / M)``; rows before ``o`` get the codes
     ``round(code * old / new)``, the new ones ``round(x / new)`` (to the nearest code, ties to even); rows behind stay.
     A value that is not finite makes the block's scale NaN. CUDA tensors only; host slots are checked (``< Nb * P``,
-    and the rule above), a CUDA tensor is trusted (slots outside the pool are passed over). The pools must not overlap. No
-    counterpart in the reference."""
-    index = k_pool.get_device() if isinstance(k_pool, _Tensor) else -1
-    call = None
-    if not (isinstance(k_new, _Tensor) and k_new.dtype in _STORAGE and _ready(index, k_new.dtype, k_new, v_new)
-            and k_pool.dtype in _CODES and _ready(index, k_pool.dtype, k_pool, v_pool)
-            and _ready(index, _FLOAT32, kv_scales) and _ready(index, _INT32, slots)):
-        if not _on_gpu(k_pool):
-            raise TypeError("the operators on an 8-bit cache work on CUDA tensors only")
-        call = _DeviceCall(k_new=k_new, v_new=v_new)
-        _q8_cache(call, k_pool, v_pool, kv_scales)
-    blocks, hkv, page, dim = _q8_shape(k_pool, v_pool, kv_scales)
-    shape = k_new.shape
-    if len(shape) != 3:
-        raise ValueError(f"k_new: {len(shape)}-D tensor where [N, Hkv, D] is expected")
-    if v_new.shape != shape:
-        raise ValueError(f"v_new: shape {tuple(v_new.shape)} differs from k_new's {tuple(shape)}")
-    n, nh, nd = shape
-    if nh != hkv or nd != dim:
+    and the rule above), a CUDA tensor is trusted (slots outside the pool are passed over). The pools must not overlap.
+    No counterpart in the reference."""
+    if _append_q8_native(k_pool, v_pool, kv_scales, k_new, v_new, slots):
+        return None
+    call, store, blocks, hkv, page, dim = _q8_operands(k_pool, k_pool, v_pool, kv_scales, k_new=k_new, v_new=v_new)
+    n, nh, nd = call.dims("k_new", "N Hkv D")
+    call.same_shape("v_new", "k_new")
+    if (nh, nd) != (hkv, dim):
         raise ValueError(f"k_new: [Hkv, D] = {(nh, nd)} differs from the cache's {(hkv, dim)}")
     if blocks * page > 0x7fffffff:
         raise ValueError(f"k_pool: {blocks} blocks of {page} rows are more rows than a slot can name")
-    if call is None:
-        if slots.shape != (n,):
-            _index_shape("slots", slots.shape, (n,))
-    elif _on_gpu(slots):
+    if _on_gpu(slots):
         if slots.dtype is torch.int64:               # (a slot that int32 cannot hold is outside the pool: keep it there)
             slots = slots.clamp(-1, 0x7fffffff)
-        slots = call.index("slots", _whole("slots", slots), (n,), blocks * page, False)
+        where = call.index("slots", _whole("slots", slots), (n,), blocks * page, False)
     else:
-        slots = torch.from_numpy(_host_slots(slots, n, blocks, page)).to(call.device)
+        where = torch.from_numpy(_host_slots(slots, n, blocks, page)).to(call.device)
     if n:
-        _run(index, _fusedtok._lib.fusedtok_kv_append_paged_q8_launch, _STORAGE[k_new.dtype][1], _CODES[k_pool.dtype],
-             k_new.data_ptr(), v_new.data_ptr(), slots.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
-             kv_scales.data_ptr(), n, hkv, dim, page, blocks)
+        call.launch(_fusedtok.kv_append_paged_q8_launch, call.code, store, k_new.data_ptr(), v_new.data_ptr(),
+                    where.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), kv_scales.data_ptr(), n, hkv, dim, page,
+                    blocks)
     return None
 
 
@@ -758,30 +701,21 @@ class BlockTableStep(NamedTuple):
     free_count: object
 
 
-def _table_operands(page, block_table, lens, change, free_blocks, free_count, change_name):
-    """Check the operands of a block table operator: contiguous int32 CUDA tensors of one device (they hold the state of
-    the cache, so nothing is converted). Returns (device index, B, S)."""
-    index = block_table.get_device() if isinstance(block_table, _Tensor) else -1
-    if not _ready(index, _INT32, block_table, lens, change, free_blocks, free_count):
-        if not _on_gpu(block_table):
-            raise TypeError("the block table operators work on CUDA tensors only")
-        _DeviceCall(dtypes=(_INT32,), **{"block_table": block_table, "lens": lens, change_name: change,
-                                         "free_blocks": free_blocks, "free_count": free_count})
-    shape = block_table.shape
-    if len(shape) != 2:
-        _index_shape("block_table", shape, (None, None))
-    b, width = shape
-    if lens.shape != (b,):
-        _index_shape("lens", lens.shape, (b,))
-    if change.shape != (b,):
-        _index_shape(change_name, change.shape, (b,))
-    if len(free_blocks.shape) != 1:
-        _index_shape("free_blocks", free_blocks.shape, (None,))
-    if free_count.shape != (1,):
-        _index_shape("free_count", free_count.shape, (1,))
+def _table_operands(block_table, page, **rest):
+    """Operands of the block table operators: contiguous int32 CUDA tensors of one device (they hold the state of the
+    cache, so nothing is converted). Returns (call, B, S)."""
+    if not _on_gpu(block_table):
+        raise TypeError("the block table operators work on CUDA tensors only")
+    call = _DeviceCall(dtypes=(torch.int32,), block_table=block_table, **rest)
+    b, width = call.dims("block_table", "B S")
+    for name in ("lens", "new_lens", "keep_lens"):
+        if name in rest:
+            _index_shape(name, rest[name].shape, (b,))
+    _index_shape("free_blocks", rest["free_blocks"].shape, (None,))
+    _index_shape("free_count", rest["free_count"].shape, (1,))
     if not isinstance(page, (int, np.integer)) or page < 1:
         raise ValueError(f"page {page}: blocks of a whole number of rows, at least one, are required")
-    return index, b, width
+    return call, b, width
 
 
 def block_table_extend(block_table, lens, new_lens, free_blocks, free_count, page, max_tokens):
@@ -796,17 +730,18 @@ def block_table_extend(block_table, lens, new_lens, free_blocks, free_count, pag
     get slot -1. So is the first one that the free stack cannot serve, and every later one that needs a block. All
     tensors are contiguous int32 CUDA tensors (at most 8192 sequences), read on the GPU and trusted; free_blocks and
     free_count are not changed - give the returned count to the next call. No counterpart in the reference."""
-    index, b, width = _table_operands(page, block_table, lens, new_lens, free_blocks, free_count, "new_lens")
+    step = _extend_native(block_table, lens, new_lens, free_blocks, free_count, page, max_tokens)
+    if step is not None:
+        return step
+    call, b, width = _table_operands(block_table, page, lens=lens, new_lens=new_lens, free_blocks=free_blocks,
+                                     free_count=free_count)
     if not isinstance(max_tokens, (int, np.integer)) or not 0 <= max_tokens <= 0x7fffffff:
         raise ValueError(f"max_tokens {max_tokens}: a count of tokens below 2^31 is expected")
-    n = int(max_tokens)
-    made = lens.new_empty(n + 2 * b + 2)                 # one allocation for the four results
-    step = BlockTableStep(*made.split_with_sizes([n, b + 1, b, 1]))
-    at = made.data_ptr()
-    _run(index, _fusedtok._lib.fusedtok_block_table_extend_launch, block_table.data_ptr(), lens.data_ptr(),
-         new_lens.data_ptr(), free_blocks.data_ptr(), free_count.data_ptr(), at, at + 4 * n, at + 4 * (n + b + 1),
-         at + 4 * (n + 2 * b + 1), b, width, int(page), free_blocks.shape[0], n)
-    return step
+    slots, starts, lens_out, left = (call.new((k,)) for k in (int(max_tokens), b + 1, b, 1))
+    call.launch(_fusedtok.block_table_extend_launch, block_table.data_ptr(), lens.data_ptr(), new_lens.data_ptr(),
+                free_blocks.data_ptr(), free_count.data_ptr(), slots.data_ptr(), starts.data_ptr(),
+                lens_out.data_ptr(), left.data_ptr(), b, width, int(page), free_blocks.shape[0], int(max_tokens))
+    return BlockTableStep(slots, starts, lens_out, left)
 
 
 def block_table_trim(block_table, lens, keep_lens, free_blocks, free_count, page):
@@ -814,9 +749,33 @@ def block_table_trim(block_table, lens, keep_lens, free_blocks, free_count, page
     tokens) and push the blocks that they no longer need on the free stack, in batch order, from
     ``free_blocks[free_count]`` on. Returns ``(lens, free_count)``, the new lengths and count; the table is only read.
     Operands as in :func:`block_table_extend`. No counterpart in the reference."""
-    index, b, width = _table_operands(page, block_table, lens, keep_lens, free_blocks, free_count, "keep_lens")
-    lens_out, left = lens.new_empty(b), lens.new_empty(1)
-    _run(index, _fusedtok._lib.fusedtok_block_table_trim_launch, block_table.data_ptr(), lens.data_ptr(),
-         keep_lens.data_ptr(), free_blocks.data_ptr(), free_count.data_ptr(), lens_out.data_ptr(), left.data_ptr(), b,
-         width, int(page), free_blocks.shape[0])
+    cut = _trim_native(block_table, lens, keep_lens, free_blocks, free_count, page)
+    if cut is not None:
+        return cut
+    call, b, width = _table_operands(block_table, page, lens=lens, keep_lens=keep_lens, free_blocks=free_blocks,
+                                     free_count=free_count)
+    lens_out, left = call.new((b,)), call.new((1,))
+    call.launch(_fusedtok.block_table_trim_launch, block_table.data_ptr(), lens.data_ptr(), keep_lens.data_ptr(),
+                free_blocks.data_ptr(), free_count.data_ptr(), lens_out.data_ptr(), left.data_ptr(), b, width,
+                int(page), free_blocks.shape[0])
     return lens_out, left
+
+
+# ---------------------------------------------------------------------------
+# plain calls without the detour through this file
+# ---------------------------------------------------------------------------
+
+try:
+    from . import _tensors
+except ImportError:          # not built, or built for another torch
+    _tensors = None
+else:
+    _tensors.bind(*_fusedtok.addresses(
+        "fusedtok_last_error", "fusedtok_attention_decode_paged_q8_workspace", "fusedtok_attention_decode_paged_q8_launch",
+        "fusedtok_kv_append_paged_q8_launch", "fusedtok_block_table_extend_launch", "fusedtok_block_table_trim_launch"),
+        BlockTableStep)
+
+_decode_q8_native = _native("attention_decode_paged_q8")
+_append_q8_native = _native("kv_append_paged_q8")
+_extend_native = _native("block_table_extend")
+_trim_native = _native("block_table_trim")

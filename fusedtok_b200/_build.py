@@ -10,6 +10,7 @@ import os
 import re
 import subprocess
 import sys
+import sysconfig
 import time
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -92,9 +93,47 @@ def _compile(variants, force=False, verbose=False):
         os.utime(target, (began, began))
 
 
+# The module that makes plain calls straight from torch tensors (csrc/tensor_calls.cpp). An accelerator of the Python
+# wrappers, not another way to compute: without it every call takes the wrappers' way.
+BINDING = os.path.join(HERE, "_tensors.so")
+
+
+def build_binding(force=False):
+    """Compile the module with the C++ headers of the installed torch; nothing to do without torch."""
+    source = os.path.join(CSRC, "tensor_calls.cpp")
+    stamp = os.path.join(OBJECTS, "tensor_calls.torch")      # the torch it was built for
+    try:
+        import torch
+        from torch.utils import cpp_extension
+    except ImportError:
+        return None
+    built_for = open(stamp).read() if os.path.exists(stamp) else ""
+    if not force and built_for == torch.__version__ and not _out_of_date(BINDING, source):
+        return BINDING
+    began = time.time()
+    root = os.path.dirname(torch.__file__)
+    cuda = os.environ.get("CUDA_HOME") or cpp_extension.CUDA_HOME or "/usr/local/cuda"
+    cmd = ["g++", "-O2", "-std=c++20", "-fPIC", "-shared", source, "-o", BINDING]
+    for d in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+              os.path.join(cuda, "include"), sysconfig.get_paths()["include"]):
+        cmd += ["-I", d]
+    cmd += ["-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    if subprocess.call(cmd) != 0:
+        if os.path.exists(BINDING):
+            os.remove(BINDING)
+        print("fusedtok_b200: %s was not built; calls take the Python wrappers' way" % BINDING)
+        return None
+    os.utime(BINDING, (began, began))
+    os.makedirs(OBJECTS, exist_ok=True)
+    with open(stamp, "w") as f:
+        f.write(torch.__version__)
+    return BINDING
+
+
 def build_all(force=False):
     """The product and the self-checking variant, whichever is out of date, compiled side by side."""
     _compile([(d, t) for d, t in (((), LIB), (("FTK_BOUNDS",), BOUNDS_LIB)) if force or stale(t)], force)
+    build_binding(force)
     return LIB
 
 
@@ -103,6 +142,8 @@ def build(force=False, verbose=False, defines=(), out=None):
     ``defines=["FTK_TIMELINE"]``: per-CTA timestamps in the tensor-core decode kernel, read back with
     ``ftk_debug_timeline``); the product itself is always built without defines."""
     target = out or LIB
+    if not defines:
+        build_binding(force)
     if not force and not defines and not stale():
         return LIB
     _compile([(tuple(defines), target)], force, verbose)

@@ -117,6 +117,11 @@ def _check(rc):
     raise RuntimeError(msg)
 
 
+def addresses(*names):
+    """Addresses of entry points of the loaded library, for other native code that is to call this very build."""
+    return [ctypes.cast(getattr(_lib, n), _vp).value for n in names]
+
+
 def _opt(p):
     return None if (p is None or p == 0) else int(p)
 

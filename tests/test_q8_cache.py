@@ -734,6 +734,40 @@ def test_captured_steps_on_two_streams(page, dim):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("page,dim", [(16, 128), (12, 64)])
+def test_plain_calls_and_the_careful_way_agree(page, dim, monkeypatch):
+    """The module that takes plain calls straight to the library is there, takes them, and does what the wrappers do; what it
+    does not take reaches them."""
+    f = ft()
+    assert f._tensors is not None
+    native, careful = _step_state(21, page, dim), _step_state(21, page, dim)
+    a = [_decode_step(native).clone() for _ in range(4)]
+    names = ("_decode_q8_native", "_append_q8_native", "_extend_native", "_trim_native")
+    taken = []
+    for n in names:
+        monkeypatch.setattr(f, n, lambda *x, n=n, real=getattr(f, n): taken.append((n, real(*x) is not None)))
+    b = []
+    for _ in range(4):
+        plan = f.block_table_extend(careful["table"], careful["lens"], careful["ones"], careful["free"], careful["count"], page, 5)
+        f.kv_append_paged_q8(careful["k"], careful["v"], careful["s"], careful["x"], careful["x"], plan.slots)
+        b.append(f.attention_decode_paged_q8(careful["q"], careful["k"], careful["v"], careful["s"], careful["table"], plan.lens))
+        assert type(plan) is f.BlockTableStep and plan.starts.tolist() == [0, 1, 2, 3, 4, 5]
+        careful["lens"], careful["count"] = plan.lens, plan.free_count
+    assert taken == [(n, True) for n in ("_extend_native", "_append_q8_native", "_decode_q8_native")] * 4
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+    for key in ("k", "v", "s", "table", "lens", "count"):
+        assert torch.equal(native[key].view(torch.uint8), careful[key].view(torch.uint8)), key
+    monkeypatch.undo()
+    keep = native["lens"] // 2
+    one, two = native["free"].clone(), native["free"].clone()
+    cut = f.block_table_trim(native["table"], native["lens"], keep, one, native["count"], page)
+    monkeypatch.setattr(f, "_trim_native", lambda *x: None)
+    again = f.block_table_trim(native["table"], native["lens"], keep, two, native["count"], page)
+    assert all(torch.equal(x, y) for x, y in zip(cut, again)) and torch.equal(one, two)
+
+
+@pytest.mark.gpu
 def test_same_bits_every_call():
     rng = np.random.default_rng(2)
     lens = [3000, 17, 900]

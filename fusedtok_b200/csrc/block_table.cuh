@@ -8,9 +8,10 @@
 // trim: the blocks behind ceil(keep / P) go back, in batch order, to free[free_count], free[free_count + 1], ...
 //
 // A few hundred bytes to a megabyte move; what counts is latency. One launch each: every CTA works out the prefix sums
-// of the whole batch for itself in shared memory (up to BT_MAX_BATCH sequences, one block-wide scan of two sums per
-// BT_THREADS sequences), which spares a second launch or a barrier across the grid, and then takes its share of the
-// outputs, counted in table entries and slots: whose they are is found by binary search in the sums.
+// of the whole batch for itself in shared memory (up to BT_MAX_BATCH sequences: consecutive ones per thread, one block-wide
+// scan of two sums; a scan per BT_THREADS sequences took 2048 of them 6.6 us), which spares a second launch or a barrier
+// across the grid, and then takes its share of the outputs, counted in table entries and slots: whose they are is found by
+// binary search in the sums.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -85,36 +86,47 @@ __global__ void __launch_bounds__(BT_THREADS) block_table_extend_kernel(const Bl
     const long long room = (long long)p.width * p.page;
     const int count = min(max(__ldg(p.free_count), 0), p.capacity);
     if (tid == 0) { s_taken = 0; s_start[0] = 0; }
-    long long tokens = 0, asked = 0;
-    for (int base = 0; base < p.B; base += BT_THREADS) {
-        const int b = base + tid;
-        const long long len = b < p.B ? max(__ldg(p.lens + b), 0) : 0;
-        const long long add = b < p.B ? max(__ldg(p.change + b), 0) : 0;
-        const bool row_fits = len + add <= room;
-        bool fits = row_fits;
-        int ask = fits ? bt_blocks(len + add, p.page) - bt_blocks(len, p.page) : 0;
-        Sums all, upto = bt_scan(Sums{add, ask}, red, all);
-        if (tokens + all.a > p.max_tokens) {
-            // some sequence here has tokens behind the slot map's end and asks for nothing: the second sum again
-            fits = row_fits && tokens + upto.a <= p.max_tokens;
-            if (!fits) ask = 0;
-            upto = bt_scan(Sums{add, ask}, red, all);
-        }
-        upto.a += tokens;
-        upto.b += asked;
-        const bool granted = fits && (ask == 0 || upto.b <= count);
-        if (granted && ask) atomicMax(&s_taken, (int)upto.b);          // (who is granted blocks comes before who is not)
-        if (b < p.B) {
-            s_start[b + 1] = (int)min(upto.a, 0x7fffffffll);
-            s_off[b] = (int)min(upto.b - ask, 0x7fffffffll) | (granted ? 0 : BT_REFUSED);
-            if (blockIdx.x == 0) {
-                p.starts[b + 1] = s_start[b + 1];
-                p.lens_out[b] = (int)(granted ? len + add : len);
-            }
-        }
-        tokens += all.a;
-        asked += all.b;
+    // this thread's sequences [b0, b1), one after the other: f(b, tokens held, tokens to add)
+    const int each = (p.B + BT_THREADS - 1) / BT_THREADS;
+    const int b0 = min(tid * each, p.B), b1 = min(b0 + each, p.B);
+    auto sequences = [&](auto f) {
+#pragma unroll 4
+        for (int b = b0; b < b1; ++b) f(b, (long long)max(__ldg(p.lens + b), 0), (long long)max(__ldg(p.change + b), 0));
+    };
+    auto missing = [&](long long len, long long add) { return bt_blocks(len + add, p.page) - bt_blocks(len, p.page); };
+    Sums mine{0, 0}, all;
+    sequences([&](int, long long len, long long add) {
+        mine.a += add;
+        if (len + add <= room) mine.b += missing(len, add);
+    });
+    Sums before = bt_scan(mine, red, all);
+    before.a -= mine.a;
+    if (all.a > p.max_tokens) {
+        // some sequences have tokens behind the slot map's end and ask for nothing: the second sum again
+        long long end = before.a;
+        mine.b = 0;
+        sequences([&](int, long long len, long long add) {
+            end += add;
+            if (len + add <= room && end <= p.max_tokens) mine.b += missing(len, add);
+        });
+        before.b = bt_scan(Sums{0, mine.b}, red, all).b;
     }
+    before.b -= mine.b;
+    sequences([&](int b, long long len, long long add) {
+        before.a += add;
+        const bool fits = len + add <= room && before.a <= p.max_tokens;
+        const int ask = fits ? missing(len, add) : 0;
+        const long long upto = before.b + ask;
+        const bool granted = fits && (ask == 0 || upto <= count);
+        if (granted && ask) atomicMax(&s_taken, (int)upto);            // (who is granted blocks comes before who is not)
+        s_start[b + 1] = (int)min(before.a, 0x7fffffffll);
+        s_off[b] = (int)min(before.b, 0x7fffffffll) | (granted ? 0 : BT_REFUSED);
+        before.b = upto;
+        if (blockIdx.x == 0) {
+            p.starts[b + 1] = s_start[b + 1];
+            p.lens_out[b] = (int)(granted ? len + add : len);
+        }
+    });
     __syncthreads();
     const int taken = s_taken;
     if (blockIdx.x == 0 && tid == 0) {
@@ -174,23 +186,25 @@ __global__ void __launch_bounds__(BT_THREADS) block_table_trim_kernel(const Bloc
     const int tid = threadIdx.x;
     const long long room = (long long)p.width * p.page;
     const int count = min(max(__ldg(p.free_count), 0), p.capacity);
-    long long gone = 0;
-    for (int base = 0; base < p.B; base += BT_THREADS) {
-        const int b = base + tid;
-        int keep = 0, back = 0;
-        if (b < p.B) {
+    const int each = (p.B + BT_THREADS - 1) / BT_THREADS;
+    const int b0 = min(tid * each, p.B), b1 = min(b0 + each, p.B);
+    auto sequences = [&](auto f) {                     // f(b, tokens kept, blocks given back)
+#pragma unroll 4
+        for (int b = b0; b < b1; ++b) {
             const int len = (int)min((long long)max(__ldg(p.lens + b), 0), room);
-            keep = min(max(__ldg(p.change + b), 0), len);
-            back = bt_blocks(len, p.page) - bt_blocks(keep, p.page);
+            const int keep = min(max(__ldg(p.change + b), 0), len);
+            f(b, keep, bt_blocks(len, p.page) - bt_blocks(keep, p.page));
         }
-        Sums all;
-        const Sums upto = bt_scan(Sums{back, 0}, red, all);
-        if (b < p.B) {
-            s_off[b] = (int)min(gone + upto.a - back, 0x7fffffffll);
-            if (blockIdx.x == 0) p.lens_out[b] = keep;
-        }
-        gone += all.a;
-    }
+    };
+    Sums mine{0, 0}, all;
+    sequences([&](int, int, int back) { mine.a += back; });
+    long long before = bt_scan(mine, red, all).a - mine.a;
+    const long long gone = all.a;
+    sequences([&](int b, int keep, int back) {
+        s_off[b] = (int)min(before, 0x7fffffffll);
+        before += back;
+        if (blockIdx.x == 0) p.lens_out[b] = keep;
+    });
     const int pushed = (int)min(gone, (long long)(p.capacity - count));      // (a stack that is full takes no more)
     if (blockIdx.x == 0 && tid == 0) *p.count_out = count + pushed;
     __syncthreads();

@@ -7,15 +7,21 @@
 // the scales never touch the codes: ks multiplies the finished score, vs is folded into the softmax weight.
 //
 // Structure (see decode_tc.cuh for the parts both share): one persistent CTA per SM; all tiles of all units cut at equal
-// cost into one range per CTA, worked out on the device from lens. Three kinds of warps, every one walking the range for
+// cost into one range per CTA, worked out on the device from lens. Four kinds of warps, every one walking the range for
 // itself:
-//  * 4 producer warps stream 64-row tiles with TMA into a ring in shared memory, one for each group of consumer warps;
-//  * 8 consumer warps, in 4 groups that take tiles in turn, keep an online softmax over their rows in registers. Nothing
-//    makes them meet: at the end of a segment (the range's part of a unit) a warp leaves its state (m, l, O) in a buffer
-//    and goes on;
+//  * 4 producer warps stream 64-row tiles with TMA into a ring in shared memory, every fourth tile each;
+//  * 8 consumer warps, in groups of two that take tiles in turn, keep an online softmax over their rows in registers.
+//    Nothing makes them meet: at the end of a segment (the range's part of a unit) a warp leaves its state (m, l, O) in a
+//    buffer and goes on;
 //  * 2 helper warps prepare the query fragments of the next segments, 2 fold the 8 states of the last ones. With both done
 //    by the consumers, and barriers between them, every segment cost a CTA about 4 us (12 tiles' worth), and 64 ragged
-//    sequences took 130 us instead of 95.
+//    sequences took 130 us instead of 90.
+// Measured (B200, back to back in a graph, 3 % more under sustained power): 32 sequences x 4096 rows, 32 / 8 heads of 128,
+// bf16 and int8: 49.5 us, 5.4 TB/s; 64 ragged ones of 128 - 8192 rows, fp16 and e4m3: 89 us, 6.1 TB/s; 4 x 131072 rows, 64 / 8
+// heads, bf16 and e4m3: 164 us, 6.5 TB/s, the copy rate. What is left of the first is its ends: 3.3 us from the release of
+// the launch to the first copy (lengths read, ranges located, table entries read), 1.5 us from a CTA's last tile to its
+// exit, 2.7 us for the merge behind. Consumers are the limit from 16 heads per kv head (68 us) and, with 16-row blocks of
+// 64-wide heads, the rate of 1 KB copies (60 us; 52 us with 64-row blocks).
 //  * Stage layout: a block's (page x D) bytes are contiguous in the pool, so the pool is described to TMA as 128-byte
 //    lines with the 128-byte swizzle, whatever D is; row r, 16-byte chunk c of a tile sits at line-linear address
 //    r * D + 16 c, swizzled. One copy per block and tile for K, one for V; the two scales of the block follow with an
@@ -27,8 +33,8 @@
 //    its upper half and the odd d in its lower half.
 //  * Weights: with |vs| = c * 2^e, 1 <= c < 2, the running maximum R is that of s + e (log2 units) and the weight
 //    w = 2^(s + e - R) lies in [0, 1]: the MMA gets w * c, rounded to half relative to the largest CONTRIBUTION so far, and
-//    l += w * 2^-e, the sum of 2^(s - R), stays in fp32. e is counted from a warp's first block, so that both stay in
-//    range as long as the V scales of a sequence differ by less than 2^60; scales below 2^-126 count as 0.
+//    l += w * 2^-e, the sum of 2^(s - R), stays in fp32. e is counted from a warp's first block that is not zero, so that
+//    both stay in range as long as the V scales of a sequence differ by less than 2^60.
 //  * SPLIT: with at most 4 query heads per unit (8 with two column blocks) each head takes two of the 8 MMA columns, the
 //    value rounded to half and the remainder: q and P' then carry 22 bits at no cost in MMAs. float32 calls always run
 //    this way (that is what keeps them at float32 accuracy on half-precision tensor cores), 16-bit calls when their
@@ -542,7 +548,10 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 #pragma unroll
         for (int n = 0; n < PF; ++n) ldsm_x4_t(st_v + chunk_off(n / NLD, n % NLD), f[n][0], f[n][1], f[n][2], f[n][3]);
         // ---- online softmax, in units of log2
-        if (e0 < 0) e0 = (int)min(max((__float_as_uint(ks[0].y) >> 23) & 255u, 64u), 190u);
+        if (e0 < 0) {
+            const unsigned int e = (__float_as_uint(ks[0].y) >> 23) & 255u;
+            e0 = e ? (int)min(max(e, 64u), 190u) : 127;        // (a block of zeros says nothing about the others)
+        }
         float de[RB], ge[RB], ce[RB];    // per block: exponent of vs less e0, 2^-that, and what is left of vs
 #pragma unroll
         for (int j = 0; j < RB; ++j) {
@@ -883,7 +892,7 @@ decode_q8_generic_kernel(const Q8Params p) {
 // kernel and ends in a later one, if any: its first partial is slot 2 c + 1, the next ones the even slots behind.
 // Otherwise block u folds the nsplit slots of unit u of the generic kernel. All latency: the (m, l) of up to 32 partials and
 // the first sums of each thread's are requested together; 4 teams of threads take every fourth partial, and their sums
-// are added in order.
+// are added in order (one team: 1.5 us more with 19 partials; 2 or 8: 0.6 us more).
 constexpr int Q8M_TEAMS = 4, Q8M_TEAM = 128, Q8M_THREADS = Q8M_TEAMS * Q8M_TEAM;
 template <bool TC>
 __global__ void __launch_bounds__(Q8M_THREADS) q8_merge_kernel(const Q8Params p) {

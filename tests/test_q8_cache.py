@@ -258,6 +258,24 @@ def test_decode_scales_of_any_size(dim, page, store):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("store", list(STORES))
+@pytest.mark.parametrize("dim,page", [(128, 16), (64, 64)])
+@pytest.mark.parametrize("big", [2.0 ** 40, 2.0 ** -40])
+def test_decode_blocks_of_zeros(dim, page, store, big):
+    """Blocks of zeros (scale 0) at the head of a sequence and all over it, among blocks of very large or very small values."""
+    rng = np.random.default_rng(17)
+    lens = [page * 20 + 3, page * 3, page * 2 + 1]
+    k, v, scales, table = make_cache(rng, lens, 2, dim, page, store)
+    scales[..., 1] *= np.float32(big)
+    scales[table[0, :8], :, 1] = 0
+    scales[table[1, :3], :, 1] = 0
+    scales[table[2, 1:], 0, 1] = 0
+    q = rounded(rng.standard_normal((3, 8, dim)), "f32")
+    got = check_decode(q, k, v, scales, table, lens, store, "f32")
+    assert not got[1].any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dim,page", [(128, 16), (64, 12)])
 def test_decode_nan_stays_in_its_heads(dim, page):
     rng = np.random.default_rng(8)

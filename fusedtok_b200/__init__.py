@@ -713,8 +713,8 @@ def _table_operands(block_table, page, **rest):
             _index_shape(name, rest[name].shape, (b,))
     _index_shape("free_blocks", rest["free_blocks"].shape, (None,))
     _index_shape("free_count", rest["free_count"].shape, (1,))
-    if not isinstance(page, (int, np.integer)) or page < 1:
-        raise ValueError(f"page {page}: blocks of a whole number of rows, at least one, are required")
+    if not isinstance(page, (int, np.integer)) or not 1 <= page <= 0x7fffffff:
+        raise ValueError(f"page {page}: blocks of a whole number of rows, at least one and below 2^31, are required")
     return call, b, width
 
 
@@ -767,7 +767,9 @@ def block_table_trim(block_table, lens, keep_lens, free_blocks, free_count, page
 
 try:
     from . import _tensors
-except ImportError:          # not built, or built for another torch
+    if torch is None or torch.__version__.split("+")[0] != _tensors.torch_version:
+        raise ImportError("built for another torch")
+except ImportError:          # not built, or not for this torch
     _tensors = None
 else:
     _tensors.bind(*_fusedtok.addresses(

@@ -286,6 +286,7 @@ int fusedtok_kv_append_paged_q8_launch(int dtype, int store, const void* k_new, 
     if (dim % 4 != 0 || dim > 512) return fail(FUSEDTOK_INVALID_ARGUMENT, "dim must be a multiple of 4 and at most 512");
     if (page < 1) return fail(FUSEDTOK_INVALID_ARGUMENT, "page size must be >= 1");
     if (num_blocks * page > 0x7fffffffll) return fail(FUSEDTOK_INVALID_ARGUMENT, "the pool has more rows than a slot can name");
+    if ((long long)page * dim > 0x7fffffffll) return fail(FUSEDTOK_INVALID_ARGUMENT, "a block's rows of one head must be below 2^31 bytes");
     if (tokens == 0 || num_blocks == 0) return FUSEDTOK_OK;
     if (!k_new || !v_new || !slots || !k_pool || !v_pool || !kv_scales) return fail(FUSEDTOK_INVALID_ARGUMENT, "null kv append operand");
     const size_t es = dtype == 0 ? 4 : 2;

@@ -18,6 +18,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/version.h>
 #include <ATen/ops/empty.h>
 
 #include "../../include/fusedtok_b200.h"
@@ -244,4 +245,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensors", nullptr, -1, methods, n
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__tensors() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__tensors() {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "torch_version", TORCH_VERSION) < 0) Py_CLEAR(m);      // whose classes it was built for
+    return m;
+}

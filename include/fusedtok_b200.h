@@ -320,7 +320,8 @@ int fusedtok_attention_decode_launch_noalloc(int dtype, const void* q, const voi
  * Rows behind the run keep their codes (they stand for nothing until they are
  * appended). new == 0 gives codes 0; a NaN or infinity among the run's values
  * makes the scale NaN, and the block reads as NaN until it is begun again at
- * offset 0. D % 4 == 0, D <= 512, Nb * P < 2^31; the two pools must not overlap. */
+ * offset 0. D % 4 == 0, D <= 512, Nb * P < 2^31, P * D < 2^31; the two pools must
+ * not overlap. */
 long long fusedtok_attention_decode_paged_q8_workspace(int dtype, int batch, int q_heads, int kv_heads, int page,
                                                        int tbl_width, int dim);
 int fusedtok_attention_decode_paged_q8_launch(int dtype, int store, const void* q, const void* k_pool,
@@ -370,9 +371,10 @@ int fusedtok_block_table_trim_launch(const int* table, const int* lens, const in
  * a non-zero code in a per-device status word and the kernel still completes.
  * This call synchronises the current device, returns the word through
  * `status` (0 = ok) and clears it. It covers both the workspace the allocating
- * launchers own and the static scratch of the allocation-free launcher (the
- * first non-zero of the two is returned), and the 8-bit decode's own word; after a non-zero word the arrival
- * counters of that path are cleared too, so the next launch starts clean. */
+ * launchers own, the static scratch of the allocation-free launcher and the
+ * 8-bit decode's own word (the first non-zero one is returned); after a non-zero
+ * word of the first two the arrival counters of that path are cleared too, so the
+ * next launch starts clean. */
 int fusedtok_attention_device_status(int* status);
 
 /* Number of kernels this library has launched on this thread since the last

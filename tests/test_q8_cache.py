@@ -119,6 +119,29 @@ def test_launchers_refuse_before_touching_the_gpu():
             lib.block_table_trim_launch(**{**good, **change})
 
 
+def test_append_refuses_blocks_beyond_32_bits():
+    from fusedtok_b200 import _fusedtok as lib
+    good = dict(dtype=1, store=0, k_new=64, v_new=64, slots=64, k_pool=64, v_pool=1 << 45, kv_scales=64, tokens=1, hkv=1, dim=64,
+                page=1 << 25, num_blocks=1)
+    with pytest.raises(ValueError, match="below 2\\^31 bytes"):
+        lib.kv_append_paged_q8_launch(**good)
+
+
+def test_module_of_another_torch_is_left_alone(monkeypatch):
+    """The module for plain calls binds to the torch it was built for; under another one every call takes the wrappers' way."""
+    f = ft()
+    if f._tensors is None:
+        pytest.skip("not built")
+    assert f._tensors.torch_version == torch.__version__.split("+")[0]
+    import importlib.util
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    spec = importlib.util.spec_from_file_location("fusedtok_b200", f.__file__)
+    again = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(again)
+    assert again._tensors is None
+    assert again._decode_q8_native(1, 2, 3, 4, 5, 6) is None
+
+
 def test_workspace_of_a_refused_shape():
     from fusedtok_b200 import _fusedtok as lib
     with pytest.raises(ValueError):
@@ -625,6 +648,16 @@ def test_trim(batch, page):
     run_trim(table, lens, np.where(rng.random(batch) < 0.4, 0, lens), free, 3, page)
     run_trim(table, lens, lens - rng.integers(-3, 40, batch), free, 7, page)
     run_trim(table, lens, np.zeros(batch, np.int64), free[: capacity // 2].copy(), 2, page)      # a stack that cannot hold them
+
+
+@pytest.mark.gpu
+def test_block_table_page_beyond_32_bits():
+    i = torch.zeros((2,), dtype=torch.int32, device="cuda")
+    for page in (2 ** 31, 2 ** 32 + 16):                    # (the second is 16 to 32 bits)
+        with pytest.raises(ValueError):
+            ft().block_table_extend(i.view(2, 1), i, i, i, i[:1], page, 8)
+        with pytest.raises(ValueError):
+            ft().block_table_trim(i.view(2, 1), i, i, i, i[:1], page)
 
 
 @pytest.mark.gpu

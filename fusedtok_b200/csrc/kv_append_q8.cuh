@@ -20,7 +20,7 @@
 // rounded, both out of shared memory, and no register holds data in flight. Runs of up to two slots are a warp's own, a
 // warp per pair and no barrier; longer ones the four warps share, pair by pair (up to 8 slots, a 128-row block of the same
 // rows; a run beyond that is copied twice, the second time from L2).
-// 266 k tokens of 8 x 128 half-precision values to int8 (1.64 GB): 257 us in a graph of four calls, 6390 GB/s, and 290 us
+// 266 k tokens of 8 x 128 half-precision values to int8 (1.64 GB): 257 us in a graph of four calls, 6390 GB/s, and 275 - 290 us
 // when calls follow each other for long (copies alone, without the rounding, took 277 us then). (A CTA per run: 1476 us; a
 // warp per run with its rows in registers: 546 us, 412 us with the runs of a window found at once.) 256 tokens of one step:
 // 7.2 us, 32 tokens 3.5 us: a chain of dependent loads for the first token of a warp, 2 us of instructions for each further one.

@@ -892,7 +892,8 @@ decode_q8_generic_kernel(const Q8Params p) {
 // kernel and ends in a later one, if any: its first partial is slot 2 c + 1, the next ones the even slots behind.
 // Otherwise block u folds the nsplit slots of unit u of the generic kernel. All latency: the (m, l) of up to 32 partials and
 // the first sums of each thread's are requested together; 4 teams of threads take every fourth partial, and their sums
-// are added in order (one team: 1.5 us more with 19 partials; 2 or 8: 0.6 us more).
+// are added in order (one team: 1.5 us more with 19 partials; 2 or 8: 0.6 us more). gridDim.y blocks share a unit's sums,
+// 128 float4 at a time.
 constexpr int Q8M_TEAMS = 4, Q8M_TEAM = 128, Q8M_THREADS = Q8M_TEAMS * Q8M_TEAM;
 template <bool TC>
 __global__ void __launch_bounds__(Q8M_THREADS) q8_merge_kernel(const Q8Params p) {
@@ -919,7 +920,8 @@ __global__ void __launch_bounds__(Q8M_THREADS) q8_merge_kernel(const Q8Params p)
     const int team = tid / Q8M_TEAM, at = tid % Q8M_TEAM;
     const int quads = p.D >> 2, items = gv * quads;
     if (tid < 16) { s_top[tid] = -INFINITY; s_l[tid] = 0.0f; }
-    for (int i0 = 0; i0 < items; i0 += Q8M_TEAM) {
+    const int i_first = (int)blockIdx.y * Q8M_TEAM;
+    for (int i0 = i_first; i0 < items; i0 += (int)gridDim.y * Q8M_TEAM) {
         const int it = i0 + at;
         const int g = it < items ? it / quads : 0, d = it < items ? (it - g * quads) * 4 : 0;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -935,7 +937,7 @@ __global__ void __launch_bounds__(Q8M_THREADS) q8_merge_kernel(const Q8Params p)
                 v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (it < items && j < n) v[q] = __ldcg(reinterpret_cast<const float4*>(p.ws_acc + (slot(j0 + j) * p.GC + g) * p.D + d));
             }
-            if (i0 == 0 || parts > 32) {
+            if (i0 == i_first || parts > 32) {
                 for (int gg = warp; gg < gv; gg += Q8M_THREADS / 32) {
                     float2 ml = make_float2(-INFINITY, 0.0f);
                     if (lane < n) ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml + (slot(j0 + lane) * p.GC + gg) * 2));

@@ -237,6 +237,16 @@ def test_decode_large_batch(page, dim, store):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,dim,page,lens", [(16, 1, 128, 16, [6007]), (13, 1, 128, 16, [2500, 0, 700]), (8, 1, 256, 32, [4001]),
+                                                  (24, 1, 96, 16, [3000]), (6, 2, 112, 16, [2300]), (9, 1, 512, 16, [1500, 40])])
+def test_decode_few_units_of_many_heads(hq, hkv, dim, page, lens):
+    """Units cut into many ranges (more than 32, or not) whose merge several blocks share; last chunks of a group with fewer heads."""
+    rng = np.random.default_rng(hq * dim)
+    k, v, scales, table = make_cache(rng, lens, hkv, dim, page, "e4m3")
+    check_decode(rounded(rng.standard_normal((len(lens), hq, dim)), "f16"), k, v, scales, table, lens, "e4m3", "f16")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("page,dim", [(16, 128), (64, 64), (12, 96), (32, 256)])
 def test_decode_ignores_what_is_behind_the_end(page, dim):
     """NaN codes, infinite and NaN scales and out-of-range table entries behind the last token change nothing."""

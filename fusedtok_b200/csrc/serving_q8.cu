@@ -236,6 +236,7 @@ int fusedtok_attention_decode_paged_q8_launch(int dtype, int store, const void* 
     p.page = page; p.tbl_width = tbl_width;
     p.scale = 1.0f / sqrtf((float)dim);
     p.GC = pl.GC; p.NCH = pl.NCH; p.ncta = pl.ncta;
+    p.full = pl.ncta >= sms;
     p.box_shift = pl.box_shift; p.box_rows = 1 << pl.box_shift;
     p.scales = reinterpret_cast<const float2*>(kv_scales);
     p.blocks = num_blocks;

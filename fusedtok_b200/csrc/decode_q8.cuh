@@ -35,10 +35,13 @@
 //    w = 2^(s + e - R) lies in [0, 1]: the MMA gets w * c, rounded to half relative to the largest CONTRIBUTION so far, and
 //    l += w * 2^-e, the sum of 2^(s - R), stays in fp32. e is counted from a warp's first block that is not zero, so that
 //    both stay in range as long as the V scales of a sequence differ by less than 2^60.
-//  * SPLIT: with at most 4 query heads per unit (8 with two column blocks) each head takes two of the 8 MMA columns, the
-//    value rounded to half and the remainder: q and P' then carry 22 bits at no cost in MMAs. float32 calls always run
-//    this way (that is what keeps them at float32 accuracy on half-precision tensor cores), 16-bit calls when their
-//    heads fit.
+//  * A weight goes to the tensor cores in two halves, its value rounded to half and the remainder: 22 bits, whatever the type of
+//    q. Rounded once (2^-12 of the weight at most) it added as much error to a float16 result as the result's own rounding.
+//    SPLIT: with at most 4 query heads per unit (8 with two column blocks) each head takes two of the 8 MMA columns for the two
+//    parts of q and of the weights, at no cost in MMAs. float32 calls always run this way (q needs 22 bits too), 16-bit calls
+//    when their heads fit. Without SPLIT q, 16 bits as it is, goes in one half, and the remainders of the weights take an MMA
+//    of their own into the same accumulators: with 8 heads per kv head 53.7 us instead of 52.8 (32 x 4096 rows), with 16 79.4
+//    instead of 72.8.
 //  * A unit that lies in one range is finished in place. Otherwise the CTAs leave (m, l, acc) partials, at most two per
 //    range, in a workspace that belongs to the call, and q8_merge_kernel, launched behind with programmatic stream
 //    serialization, folds them in range order. No counters, no state between calls: calls on different streams, and
@@ -566,6 +569,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
             ce[j] = ks[j].y * __uint_as_float((uint32_t)(254 - (e0 + d)) << 23);
         }
         uint32_t pb[NBK][RB][2];
+        [[maybe_unused]] uint32_t pr[SPLIT ? 1 : NBK][RB][2];      // what the rounding to half left of the weights
 #pragma unroll
         for (int nbk = 0; nbk < NBK; ++nbk) {
             float pw[HPT][RB][2];
@@ -624,7 +628,10 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
                         const float hi = __half2float(__float2half_rn(pw[0][j][h]));
                         pb[nbk][j][h] = movmatrix_trans(pack2<__half>(hi, pw[0][j][h] - hi));
                     } else {
-                        pb[nbk][j][h] = movmatrix_trans(pack2<__half>(pw[0][j][h], pw[HPT - 1][j][h]));
+                        const uint32_t hi = pack2<__half>(pw[0][j][h], pw[HPT - 1][j][h]);
+                        const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                        pb[nbk][j][h] = movmatrix_trans(hi);
+                        pr[nbk][j][h] = movmatrix_trans(pack2<__half>(pw[0][j][h] - r.x, pw[HPT - 1][j][h] - r.y));
                     }
                 }
         }
@@ -648,8 +655,10 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
                     Codes<KV>::crossed(r[2 * half], a0, a1);
                     Codes<KV>::crossed(r[2 * half + 1], a2, a3);
 #pragma unroll
-                    for (int nbk = 0; nbk < NBK; ++nbk)
+                    for (int nbk = 0; nbk < NBK; ++nbk) {
                         mma16816<__half>(acc[nbk][mt], a0, a1, a2, a3, pb[nbk][j][0], pb[nbk][j][1]);
+                        if constexpr (!SPLIT) mma16816<__half>(acc[nbk][mt], a0, a1, a2, a3, pr[nbk][j][0], pr[nbk][j][1]);
+                    }
                 }
             }
             if (n + PF < N) ldsm_x4_t(st_v + chunk_off((n + PF) / NLD, (n + PF) % NLD), r[0], r[1], r[2], r[3]);

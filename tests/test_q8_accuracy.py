@@ -1,0 +1,73 @@
+"""Accuracy of the 8-bit decode attention, held to what float32 arithmetic gives whatever the type of q: weights and
+queries of every size, V scales of every size. The 64-bit results are those of q8_reference.py; the bound is this
+file's own (bound_of)."""
+
+import numpy as np
+import pytest
+import torch
+
+import q8_reference as ref
+import test_q8_cache as q8
+
+HALF = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}        # the result is rounded once: half a step
+
+
+def bound_of(q, k_codes, v_codes, scales, table, lens, store):
+    """(out, bound), float64 [B, Hq, D]: what the float32 result may be off by before it is rounded to the type of q.
+
+    As in q8_reference.decode_bound a score is off by at most 2^-18 of sum |q k| / sqrt(D) (natural log units) and its
+    exponential by 2^-20 more; both the numerator and the sum below it have that error. Queries go to the tensor cores
+    as halves of a row scaled into [2^14, 2^15), where what is left out is at most half a step of the smallest one, 2^-25:
+    2^-39 of the row's largest element (2^-38 here). For the product with V a weight goes in two halves, the remainder's
+    rounding being 2^-21 of the weight or less, and is scaled likewise: a small one loses at most 2^-39 (2^-38 here) of
+    the largest weight * V scale. A warp adds up at most one tensor-core step per 32 rows (generic kernel: 4 float32
+    additions with a sixteenth of the error each), each off by at most 2^-22 of the running sum of magnitudes, and the
+    partial results of up to 32 warps or ranges; so does the sum of the weights, hence 2^-21."""
+    batch, hq, dim = q.shape
+    hkv, page = k_codes.shape[1], k_codes.shape[2]
+    out, bound = np.zeros(q.shape), np.zeros(q.shape)
+    for b in range(batch):
+        n = int(lens[b])
+        if n == 0:
+            continue
+        ids = table[b, : -(-n // page)]
+        for h in range(hq):
+            kv = h // (hq // hkv)
+            k = ref.values(k_codes[ids, kv], scales[ids, kv], 0, store).reshape(-1, dim)[:n]
+            v = ref.values(v_codes[ids, kv], scales[ids, kv], 1, store).reshape(-1, dim)[:n]
+            vs = np.abs(np.repeat(scales[ids, kv, 1].astype(np.float64), page)[:n])
+            s = k @ q[b, h] / np.sqrt(dim)
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            out[b, h] = p @ v
+            size = (np.abs(k) @ np.abs(q[b, h])).max() / np.sqrt(dim)
+            left = 2.0 ** -38 * np.abs(q[b, h]).max() * np.abs(k).sum(1).max() / np.sqrt(dim)
+            d = 2.0 ** -18 * size + 2.0 ** -20 + left
+            bound[b, h] = (p @ np.abs(v)) * (2 * d + 2.0 ** -21 + (n / 32 + 32) * 2.0 ** -21) + n * 2.0 ** -38 * (p * vs).max() * ref.TOP[store]
+    return out, bound
+
+
+def check(q, k, v, scales, table, lens, store, name):
+    got = q8.ft().attention_decode_paged_q8(q.cuda(), q8.pool(k, store), q8.pool(v, store), q8.on_gpu(scales), q8.on_gpu(table),
+                                            q8.on_gpu(np.asarray(lens, np.int32)))
+    want, bound = bound_of(q.double().numpy(), k, v, scales, table, lens, store)
+    tol = bound + (np.abs(want) + bound) * HALF[name] + 2.0 ** -149       # (and the step of the smallest numbers)
+    err = np.abs(got.double().cpu().numpy() - want)
+    assert (err <= tol).all(), (float((err / tol).max()), float(err.max() / np.abs(want).max()))
+    return got
+
+
+# ---- weights ---------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("store", list(q8.STORES))
+@pytest.mark.parametrize("name", list(q8.DTYPES))
+@pytest.mark.parametrize("hq,hkv,dim,page", [(8, 2, 128, 16), (5, 1, 128, 16), (16, 2, 128, 16), (7, 1, 64, 32), (16, 1, 128, 64), (24, 1, 96, 16),
+                                             (13, 1, 80, 16), (8, 1, 192, 16), (12, 1, 256, 32), (8, 1, 112, 16), (6, 1, 64, 12)])
+def test_weights_of_any_number_of_heads(hq, hkv, dim, page, name, store):
+    """Few rows, small scores: what is left of the error is the rounding of the weights."""
+    rng = np.random.default_rng(hq * dim + page)
+    lens = [2, 17, 40, 64, 100]
+    k, v, scales, table = q8.make_cache(rng, lens, hkv, dim, page, store)
+    q = q8.rounded(0.1 * rng.standard_normal((len(lens), hq, dim)), name)
+    check(q, k, v, scales, table, lens, store, name)

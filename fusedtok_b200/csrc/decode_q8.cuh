@@ -33,7 +33,10 @@
 //    its upper half and the odd d in its lower half.
 //  * Weights: with |vs| = c * 2^e, 1 <= c < 2, the running maximum R is that of s + e (log2 units) and the weight
 //    w = 2^(s + e - R) lies in [0, 1]: the MMA gets w * c, rounded to half relative to the largest CONTRIBUTION so far, and
-//    l += w * 2^-e, the sum of 2^(s - R), stays in fp32. e is counted from a warp's first block that is not zero, so that
+//    l += w * 2^-e, the sum of 2^(s - R), stays in fp32. w * c goes in as 2^14 times itself, the most a half has room for: a
+//    weight keeps its 22 bits down to 2^-17 of the largest contribution and loses at most 2^-39 of that below. (Without the
+//    factor half precision ends at 2^-25, and thousands of rows 17 natural log units below one row, whose sum is
+//    what there is to see when that row's V is small, were lost altogether.) e is counted from a warp's first block that is not zero, so that
 //    both stay in range as long as the V scales of a sequence differ by less than 2^60.
 //  * A weight goes to the tensor cores in two halves, its value rounded to half and the remainder: 22 bits, whatever the type of
 //    q. Rounded once (2^-12 of the weight at most) it added as much error to a float16 result as the result's own rounding.
@@ -60,6 +63,7 @@ constexpr int Q8_QWARPS = 2, Q8_FWARPS = 2;     // helper warps: query fragments
 constexpr int Q8_HELPERS = Q8_QWARPS + Q8_FWARPS;
 constexpr int Q8_THREADS = (NCW + Q8_HELPERS + Q8_NP) * 32;
 static_assert(Q8_THREADS == 512, "the register split below counts 16 warps");
+constexpr float Q8_ROOM = 16384.0f;             // the largest weight goes to the tensor cores as a half between this and twice it
 constexpr int Q8_MAX_SPLIT = 32;                // generic kernel: most ranges a unit is cut into
 
 struct Q8Params : DecodeParams {
@@ -558,7 +562,8 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         // ---- online softmax, in units of log2
         if (e0 < 0) {
             const unsigned int e = (__float_as_uint(ks[0].y) >> 23) & 255u;
-            e0 = e ? (int)min(max(e, 64u), 190u) : 127;        // (a block of zeros says nothing about the others)
+            // (a block of zeros says nothing about the others; e0 + d below covers 1 .. 254, every finite scale)
+            e0 = e ? (int)min(max(e, 61u), 194u) : 127;
         }
         float de[RB], ge[RB], ce[RB];    // per block: exponent of vs less e0, 2^-that, and what is left of vs
 #pragma unroll
@@ -566,7 +571,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
             const int d = min(max((int)((__float_as_uint(ks[j].y) >> 23) & 255u) - e0, -60), 60);
             de[j] = (float)d;
             ge[j] = __uint_as_float((uint32_t)(127 - d) << 23);
-            ce[j] = ks[j].y * __uint_as_float((uint32_t)(254 - (e0 + d)) << 23);
+            ce[j] = ks[j].y * __uint_as_float(max((uint32_t)(254 - (e0 + d)) << 23, 0x00400000u)) * Q8_ROOM;
         }
         uint32_t pb[NBK][RB][2];
         [[maybe_unused]] uint32_t pr[SPLIT ? 1 : NBK][RB][2];      // what the rounding to half left of the weights
@@ -721,7 +726,8 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
             const int buf = k % Cfg::NF;
             float* s_acc = reinterpret_cast<float*>(smem + Cfg::OFF_STATE + buf * Cfg::STATE_BYTES);
             float2* s_ml = reinterpret_cast<float2*>(smem + Cfg::OFF_ML) + buf * NCW * HEADS;
-            const float unit = e0 < 0 ? 1.0f : __uint_as_float((uint32_t)e0 << 23);      // 2^e0: sums of vs * v8 again
+            // 2^e0 without the room: sums of vs * v8 again
+            const float unit = e0 < 0 ? 1.0f : __uint_as_float((uint32_t)e0 << 23) * (1.0f / Q8_ROOM);
             mbar_wait(bar_state_empty + buf * 8, (uint32_t)((k / Cfg::NF) & 1) ^ 1u, abort_flag, p.status, ST_WAIT_EMPTY_TIMEOUT);
 #pragma unroll
             for (int nbk = 0; nbk < NBK; ++nbk) {

@@ -51,7 +51,10 @@ def check(q, k, v, scales, table, lens, store, name):
     got = q8.ft().attention_decode_paged_q8(q.cuda(), q8.pool(k, store), q8.pool(v, store), q8.on_gpu(scales), q8.on_gpu(table),
                                             q8.on_gpu(np.asarray(lens, np.int32)))
     want, bound = bound_of(q.double().numpy(), k, v, scales, table, lens, store)
-    tol = bound + (np.abs(want) + bound) * HALF[name] + 2.0 ** -149       # (and the step of the smallest numbers)
+    # numbers below the smallest normal one (2^-14 in float16) have a fixed step, and rounding to it is off by half of that;
+    # the float32 result before it may be subnormal too
+    small = torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps / 2 + 2.0 ** -149
+    tol = bound + (np.abs(want) + bound) * HALF[name] + small
     err = np.abs(got.double().cpu().numpy() - want)
     assert (err <= tol).all(), (float((err / tol).max()), float(err.max() / np.abs(want).max()))
     return got
@@ -70,4 +73,26 @@ def test_weights_of_any_number_of_heads(hq, hkv, dim, page, name, store):
     lens = [2, 17, 40, 64, 100]
     k, v, scales, table = q8.make_cache(rng, lens, hkv, dim, page, store)
     q = q8.rounded(0.1 * rng.standard_normal((len(lens), hq, dim)), name)
+    check(q, k, v, scales, table, lens, store, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("store", list(q8.STORES))
+@pytest.mark.parametrize("gap", [9.0, 12.3, 15.0, 17.5, 20.0])
+@pytest.mark.parametrize("name,hq,dim,page", [("f32", 4, 128, 16), ("f32", 8, 64, 64), ("f32", 3, 256, 16), ("bf16", 16, 128, 16), ("f16", 8, 80, 16),
+                                              ("f16", 4, 128, 12)])
+def test_one_row_far_above_thousands(name, hq, dim, page, gap, store):
+    """One row whose own V is zero takes nearly all the weight; the result is what thousands of rows, `gap` natural log
+    units below it, add up to. Their V share a sign, so nothing cancels and the bound is relative to the result."""
+    rng = np.random.default_rng(int(gap * 10) + dim)
+    lens = [6007, 2500]
+    k, v, scales, table = q8.make_cache(rng, lens, 1, dim, page, store, spread=0.0)
+    full = 100.0 if store == "int8" else 104.0
+    k[:] = ref.nearest_codes(rng.integers(-2, 3, k.shape), store)
+    v[:] = ref.nearest_codes(rng.integers(64, 112, v.shape), store)
+    for b, at in enumerate((3333, 0)):
+        k[table[b, at // page], 0, at % page] = ref.nearest_codes(np.full(dim, full), store)
+        v[table[b, at // page], 0, at % page] = 0
+    scales[..., 0] = gap / (full * np.sqrt(dim))
+    q = q8.rounded(np.ones((2, hq, dim)), name)
     check(q, k, v, scales, table, lens, store, name)

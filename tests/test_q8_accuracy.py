@@ -51,9 +51,10 @@ def check(q, k, v, scales, table, lens, store, name):
     got = q8.ft().attention_decode_paged_q8(q.cuda(), q8.pool(k, store), q8.pool(v, store), q8.on_gpu(scales), q8.on_gpu(table),
                                             q8.on_gpu(np.asarray(lens, np.int32)))
     want, bound = bound_of(q.double().numpy(), k, v, scales, table, lens, store)
-    # numbers below the smallest normal one (2^-14 in float16) have a fixed step, and rounding to it is off by half of that;
-    # the float32 result before it may be subnormal too
-    small = torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps / 2 + 2.0 ** -149
+    # Numbers below the smallest normal one (2^-14 in float16) have a fixed step, and rounding to it is off by half of that.
+    # The float32 result before it may be subnormal too, and so may be every row's weight (at most 1) * V scale, whose
+    # rounding, up to 2^-150, meets a code.
+    small = torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps / 2 + 2.0 ** -149 + max(lens) * 2.0 ** -150 * ref.TOP[store]
     tol = bound + (np.abs(want) + bound) * HALF[name] + small
     err = np.abs(got.double().cpu().numpy() - want)
     assert (err <= tol).all(), (float((err / tol).max()), float(err.max() / np.abs(want).max()))
@@ -95,4 +96,25 @@ def test_one_row_far_above_thousands(name, hq, dim, page, gap, store):
         v[table[b, at // page], 0, at % page] = 0
     scales[..., 0] = gap / (full * np.sqrt(dim))
     q = q8.rounded(np.ones((2, hq, dim)), name)
+    check(q, k, v, scales, table, lens, store, name)
+
+
+# ---- V scales --------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("store", list(q8.STORES))
+@pytest.mark.parametrize("name,hq,dim,page", [("f32", 4, 128, 16), ("f32", 8, 64, 64), ("bf16", 8, 128, 16), ("f32", 2, 256, 32), ("f32", 4, 64, 12)])
+@pytest.mark.parametrize("power", [-130, -120, -90, -75, 76, 90, 115])
+def test_v_scales_of_any_size_behind_blocks_of_zeros(power, name, hq, dim, page, store):
+    """Blocks of zeros (scale 0) first, then V scales that do not differ much but are all very small (subnormal ones among
+    them) or very large: what a block of zeros is taken for must not limit the others."""
+    rng = np.random.default_rng(dim + 200 + power)
+    lens = [page * 20 + 3, page * 4, page * 3 + 1, page * 9]
+    k, v, scales, table = q8.make_cache(rng, lens, 1, dim, page, store)
+    scales[..., 1] = (scales[..., 1].astype(np.float64) * 2.0 ** power).astype(np.float32)
+    scales[table[0, :8], :, 1] = 0
+    scales[table[0, 10], :, 1] = 0
+    scales[table[1, :1], :, 1] = 0
+    scales[table[2, 1:], :, 1] = 0
+    q = q8.rounded(rng.standard_normal((4, hq, dim)), name)
     check(q, k, v, scales, table, lens, store, name)

@@ -621,9 +621,11 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
                         pw[e][j][h] = w8 * ce[j];
                     }
                 if (m_new != m_old) {
-                    const float alpha = ex2(m_old - m_safe);
+                    // in two steps for l, which may be 2^60 and more: what is left of it counts where 2^(m_old - m_new) is 0 in
+                    // float32
+                    const float half = ex2(0.5f * (m_old - m_safe)), alpha = half * half;
                     m_run[nbk][e] = m_new;
-                    l_run[nbk][e] *= alpha;
+                    l_run[nbk][e] = l_run[nbk][e] * half * half;
 #pragma unroll
                     for (int mt = 0; mt < KSTEPS; ++mt) {
                         if constexpr (SPLIT) {
@@ -750,7 +752,11 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
                     l += __shfl_xor_sync(0xffffffffu, l, 8);
                     l += __shfl_xor_sync(0xffffffffu, l, 16);
                     const int g = nbk * HB + (SPLIT ? qi : qi * 2 + e);
-                    if (quad == 0) s_ml[warp * HEADS + g] = make_float2(m_run[nbk][e], l);
+                    // Warps count V scales from different exponents. Where that has left l far from 1 (2^-60 to 2^60), its
+                    // exponent goes back into m, so that the folds, which compare m alone, lose nothing
+                    const int le = (int)(__float_as_uint(l) >> 23) - 127, k = le > 32 ? le - 32 : le < -32 ? le + 32 : 0;
+                    const float back = __uint_as_float((uint32_t)(127 - k) << 23);
+                    if (quad == 0) s_ml[warp * HEADS + g] = make_float2(m_run[nbk][e] + (float)k, l * back);
                     if (e0 != 0) {
                         float* my = s_acc + ((size_t)warp * HEADS + g) * Cfg::ACC_STRIDE + quad * 2;
 #pragma unroll
@@ -758,7 +764,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
                             float2 o;
                             if constexpr (SPLIT) o = make_float2(acc[nbk][mt][0] + acc[nbk][mt][1], acc[nbk][mt][2] + acc[nbk][mt][3]);
                             else o = make_float2(acc[nbk][mt][e], acc[nbk][mt][2 + e]);
-                            *reinterpret_cast<float2*>(my + mt * 16) = make_float2(o.x * unit, o.y * unit);
+                            *reinterpret_cast<float2*>(my + mt * 16) = make_float2(o.x * unit * back, o.y * unit * back);
                         }
                     }
                 }

@@ -118,3 +118,49 @@ def test_v_scales_of_any_size_behind_blocks_of_zeros(power, name, hq, dim, page,
     scales[table[2, 1:], :, 1] = 0
     q = q8.rounded(rng.standard_normal((4, hq, dim)), name)
     check(q, k, v, scales, table, lens, store, name)
+
+
+def rows_of_one_score(scores, v_powers, dim, store, rng):
+    """A sequence of blocks of 16 rows whose scores (log2 units, for q = 1) and V scales (powers of two; None: zero) are
+    given for each block."""
+    n = len(scores)
+    k = ref.nearest_codes(np.ones((n, 1, 16, dim)), store)
+    v = ref.nearest_codes(rng.integers(64, 112, (n, 1, 16, dim)), store)
+    scales = np.zeros((n, 1, 2), np.float32)
+    scales[:, 0, 0] = np.asarray(scores) * np.log(2.0) / np.sqrt(dim)
+    scales[:, 0, 1] = [0.0 if e is None else 2.0 ** e for e in v_powers]
+    return k, v, scales, np.arange(n, dtype=np.int32)[None]
+
+
+# (scores, V scales) block by block; a tile has four blocks, and tiles 0 and 4 meet the same warps
+FAR = [
+    # what one warp adds up with its V scales counted from the largest, and another from the smallest
+    ([-100, -7, -100, -100, -100, 0, -100, -100], [60, 0, 0, 0, 0, 60, 0, 0]),
+    ([-100, 0, -100, -100, -100, -7, -100, -100], [0, 60, 0, 0, 60, 0, 0, 0]),
+    # zeros first, then a scale far above the first that is not zero
+    ([-7, -100] + [-100] * 14 + [0, -100], [None, 0] + [0] * 14 + [60, 0]),
+    # and the other way round
+    ([-100, -100] + [-100] * 14 + [0, -7], [0, 0] + [0] * 14 + [60, None]),
+    # zeros far above everything else, and as far below
+    ([0, -20, -25, 0, -20, -30, -22, -21], [None, 0, 0, None, 0, 0, 0, 0]),
+    ([-90, 0, 0, -90, -1, -2, -3, -4], [None, 0, 0, None, 0, 0, 0, 0]),
+    # 2^60 between the scales, every order
+    ([0, 50, 60, 58, 3, 0, 0, 61] * 3, [60, 10, 0, 1, 58, 60, 59, 0] * 3),
+    ([60, 61, 59, 0, 0, 0, 55, 50] * 3, [0, 0, 1, 60, 60, 58, 5, 10] * 3),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("store", list(q8.STORES))
+@pytest.mark.parametrize("hq,dim", [(4, 128), (8, 64), (3, 256), (16, 96)])
+@pytest.mark.parametrize("case", range(len(FAR)))
+def test_v_scales_and_scores_far_apart(case, hq, dim, store):
+    """V scales that differ by 2^60, blocks of zeros, and scores that make up for it or do not: no weight that counts for the
+    sum of the weights is lost, in whichever warp it is met first."""
+    rng = np.random.default_rng(case)
+    k, v, scales, table = rows_of_one_score(*FAR[case], dim, store, rng)
+    lens = [16 * len(FAR[case][0])]
+    check(torch.ones((1, hq, dim)), k, v, scales, table, lens, store, "f32")
+    # the same blocks many times over: units that are cut, and folded by the merge
+    table = np.repeat(table, 40, axis=0).reshape(1, -1)
+    check(torch.ones((1, hq, dim)), k, v, scales, table, [16 * table.shape[1]], store, "f32")

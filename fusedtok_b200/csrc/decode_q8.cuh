@@ -189,12 +189,13 @@ __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-// Powers of two f, g with f * g = 1 and |x| * f in [1, 2) for a row's largest magnitude x (NaN for a row that is not finite).
+// Powers of two f, g with f * g = 1 and |x| * f in [2^14, 2^15) for a row's largest magnitude x (NaN for a row that is not
+// finite; f is 2^127 for x below 2^-112): as large as a half can hold, so that small elements of the row keep most bits.
 __device__ __forceinline__ void row_exponent(float x, float& f, float& g) {
-    const unsigned int e = (__float_as_uint(x) >> 23) & 255u;
-    f = e == 254u ? __uint_as_float(0x00400000u) : __uint_as_float((254u - e) << 23);
-    g = e == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(e << 23);
-    if (e == 255u) f = __uint_as_float(0x7fc00000u);
+    const int e = (int)(__float_as_uint(x) >> 23 & 255u), to = min(268 - e, 254);
+    f = __uint_as_float((uint32_t)to << 23);
+    g = to == 254 ? __uint_as_float(0x00400000u) : __uint_as_float((uint32_t)(254 - to) << 23);
+    if (e == 255) f = __uint_as_float(0x7fc00000u);
 }
 
 // ---- the kernel ----------------------------------------------------------------

@@ -99,6 +99,23 @@ def test_one_row_far_above_thousands(name, hq, dim, page, gap, store):
     check(q, k, v, scales, table, lens, store, name)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("store", list(q8.STORES))
+@pytest.mark.parametrize("name,hq,dim,page", [("f32", 4, 128, 16), ("f32", 8, 64, 64), ("bf16", 8, 128, 16), ("bf16", 2, 256, 16), ("f16", 16, 80, 16),
+                                              ("bf16", 4, 64, 12)])
+def test_queries_far_below_the_largest_of_their_row(name, hq, dim, page, store):
+    """One element of a query row is far larger than all others and meets codes that are zero: the scores are the others'."""
+    rng = np.random.default_rng(dim + hq)
+    lens = [90, 33, 5]
+    k, v, scales, table = q8.make_cache(rng, lens, 1, dim, page, store)
+    k[..., 7] = 0
+    least = 2.0 ** -10 if name == "f16" else 1.0
+    q = rng.standard_normal((3, hq, dim)) * least * 0.1
+    q[..., 7] = least * 2.0 ** (18 if name != "f16" else 25)
+    scales[..., 0] /= least
+    check(q8.rounded(q, name), k, v, scales, table, lens, store, name)
+
+
 # ---- V scales --------------------------------------------------------------------------------------------------
 
 @pytest.mark.gpu

@@ -61,6 +61,15 @@ int code_type(at::ScalarType t) { return t == at::kChar ? 0 : t == at::kFloat8_e
 bool fits_int(int64_t x) { return x <= 0x7fffffff; }
 template <typename T> T* data(const at::Tensor& t) { return static_cast<T*>(t.data_ptr()); }
 
+// Other Python threads run while a call allocates and launches: a launch waits where the stream's queue is full, which may
+// be until one of them has done its part. Nothing of Python's may be touched meanwhile.
+struct Unlocked {
+    PyThreadState* const state = PyEval_SaveThread();
+    Unlocked() = default;
+    Unlocked(const Unlocked&) = delete;
+    ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
 PyObject* declined() { Py_RETURN_NONE; }
 PyObject* failed(int rc) {
     PyErr_SetString(rc == FUSEDTOK_INVALID_ARGUMENT ? PyExc_ValueError : PyExc_RuntimeError, last_error());
@@ -112,13 +121,21 @@ PyObject* attention_decode_paged_q8(PyObject*, PyObject* const* args, Py_ssize_t
     if (b < 1 || d != cache.dim || cache.heads < 1 || hq < 1 || hq % cache.heads || table->size(0) != b || !fits_int(b) ||
         !fits_int(hq) || !fits_int(width) || (lens && lens->size(0) != b))
         return declined();
-    const long long need = decode_workspace(dtype, (int)b, (int)hq, (int)cache.heads, (int)cache.page, (int)width, (int)d);
-    if (need < 0) return failed((int)-need);
-    at::Tensor out = at::empty(q->sizes(), q->options());
-    at::Tensor scratch = at::empty({(need + 3) / 4}, cache.scales->options());
-    const int rc = decode_launch(dtype, cache.store, q->data_ptr(), cache.k->data_ptr(), cache.v->data_ptr(), data<float>(*cache.scales),
-                                 data<int>(*table), lens ? data<int>(*lens) : nullptr, out.data_ptr(), scratch.data_ptr(), need,
-                                 (int)b, (int)hq, (int)cache.heads, (int)cache.page, (int)width, cache.blocks, (int)d, in.stream());
+    at::Tensor out;
+    int rc = 0;
+    {
+        Unlocked other_threads;
+        const long long need = decode_workspace(dtype, (int)b, (int)hq, (int)cache.heads, (int)cache.page, (int)width, (int)d);
+        if (need < 0) {
+            rc = (int)-need;
+        } else {
+            out = at::empty(q->sizes(), q->options());
+            at::Tensor scratch = at::empty({(need + 3) / 4}, cache.scales->options());
+            rc = decode_launch(dtype, cache.store, q->data_ptr(), cache.k->data_ptr(), cache.v->data_ptr(), data<float>(*cache.scales),
+                               data<int>(*table), lens ? data<int>(*lens) : nullptr, out.data_ptr(), scratch.data_ptr(), need,
+                               (int)b, (int)hq, (int)cache.heads, (int)cache.page, (int)width, cache.blocks, (int)d, in.stream());
+        }
+    }
     if (rc) return failed(rc);
     return THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS
@@ -142,9 +159,13 @@ PyObject* kv_append_paged_q8(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (tokens < 1 || !fits_int(tokens) || v_new->sizes() != k_new->sizes() || k_new->size(1) != cache.heads ||
         k_new->size(2) != cache.dim || slots->size(0) != tokens)
         return declined();
-    const int rc = append_launch(dtype, cache.store, k_new->data_ptr(), v_new->data_ptr(), data<int>(*slots), cache.k->data_ptr(),
-                                 cache.v->data_ptr(), data<float>(*cache.scales), (int)tokens, (int)cache.heads, (int)cache.dim,
-                                 (int)cache.page, cache.blocks, in.stream());
+    int rc = 0;
+    {
+        Unlocked other_threads;
+        rc = append_launch(dtype, cache.store, k_new->data_ptr(), v_new->data_ptr(), data<int>(*slots), cache.k->data_ptr(),
+                           cache.v->data_ptr(), data<float>(*cache.scales), (int)tokens, (int)cache.heads, (int)cache.dim,
+                           (int)cache.page, cache.blocks, in.stream());
+    }
     if (rc) return failed(rc);
     Py_RETURN_TRUE;
     END_HANDLE_TH_ERRORS
@@ -176,11 +197,17 @@ PyObject* block_table_extend(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Table t;
     const int64_t tokens = whole(args[6], 0);
     if (tokens < 0 || !t.take(in, args)) return declined();
-    const auto options = t.lens->options();
-    at::Tensor made[4] = {at::empty({tokens}, options), at::empty({t.b + 1}, options), at::empty({t.b}, options), at::empty({1}, options)};
-    const int rc = extend_launch(data<int>(*t.table), data<int>(*t.lens), data<int>(*t.change), data<int>(*t.free_blocks),
-                                 data<int>(*t.free_count), data<int>(made[0]), data<int>(made[1]), data<int>(made[2]), data<int>(made[3]),
-                                 (int)t.b, (int)t.width, (int)t.page, (int)t.free_blocks->size(0), (int)tokens, in.stream());
+    at::Tensor made[4];
+    int rc = 0;
+    {
+        Unlocked other_threads;
+        const auto options = t.lens->options();
+        const int64_t sizes[4] = {tokens, t.b + 1, t.b, 1};
+        for (int i = 0; i < 4; ++i) made[i] = at::empty({sizes[i]}, options);
+        rc = extend_launch(data<int>(*t.table), data<int>(*t.lens), data<int>(*t.change), data<int>(*t.free_blocks),
+                           data<int>(*t.free_count), data<int>(made[0]), data<int>(made[1]), data<int>(made[2]), data<int>(made[3]),
+                           (int)t.b, (int)t.width, (int)t.page, (int)t.free_blocks->size(0), (int)tokens, in.stream());
+    }
     if (rc) return failed(rc);
     PyObject* results[4] = {nullptr, nullptr, nullptr, nullptr};
     PyObject* step = nullptr;
@@ -198,10 +225,16 @@ PyObject* block_table_trim(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Operands in;
     Table t;
     if (!t.take(in, args)) return declined();
-    at::Tensor lens = at::empty({t.b}, t.lens->options()), count = at::empty({1}, t.lens->options());
-    const int rc = trim_launch(data<int>(*t.table), data<int>(*t.lens), data<int>(*t.change), data<int>(*t.free_blocks),
-                               data<int>(*t.free_count), data<int>(lens), data<int>(count), (int)t.b, (int)t.width, (int)t.page,
-                               (int)t.free_blocks->size(0), in.stream());
+    at::Tensor lens, count;
+    int rc = 0;
+    {
+        Unlocked other_threads;
+        lens = at::empty({t.b}, t.lens->options());
+        count = at::empty({1}, t.lens->options());
+        rc = trim_launch(data<int>(*t.table), data<int>(*t.lens), data<int>(*t.change), data<int>(*t.free_blocks),
+                         data<int>(*t.free_count), data<int>(lens), data<int>(count), (int)t.b, (int)t.width, (int)t.page,
+                         (int)t.free_blocks->size(0), in.stream());
+    }
     if (rc) return failed(rc);
     PyObject* a = THPVariable_Wrap(std::move(lens));
     PyObject* c = a ? THPVariable_Wrap(std::move(count)) : nullptr;

@@ -2,6 +2,7 @@
 
 import threading
 import time
+from concurrent.futures import ThreadPoolExecutor
 
 import numpy as np
 import pytest
@@ -53,3 +54,38 @@ def test_other_threads_run_while_a_launch_waits(which):
     torch.cuda.synchronize()
     assert took[0] > 0.5                                    # it did wait
     assert longest < 0.25, longest
+
+
+@pytest.mark.parametrize("way", ["plain", "careful"])
+def test_results_of_calls_from_several_threads(way, monkeypatch):
+    """Calls that overlap on different streams, issued from different threads, give what they give alone. What a thread raises is
+    raised here, and every result is compared."""
+    if way == "careful":
+        for name in ("_decode_q8_native", "_append_q8_native"):
+            monkeypatch.setattr(q8.ft(), name, lambda *operands: None)
+    rng = np.random.default_rng(15)
+    page, dim, calls = 16, 128, 40
+    cases = []
+    for i in range(3):
+        lens = [3000 - 900 * i, 33, 500]
+        k, v, scales, table = q8.make_cache(rng, lens, 2, dim, page, "int8")
+        slots = np.array([table[b, (n - 1) // page] * page + (n - 1) % page for b, n in enumerate(lens)], np.int32)
+        cases.append(dict(k=k, v=v, s=scales, table=q8.on_gpu(table), lens=q8.on_gpu(np.array(lens, np.int32)), slots=q8.on_gpu(slots),
+                          x=q8.rounded(rng.standard_normal((calls, 3, 2, dim)), "bf16").cuda(),
+                          q=q8.rounded(rng.standard_normal((3, 8, dim)), "bf16").cuda()))
+
+    def work(c):
+        """The last token of each sequence written anew, and the attention over it, `calls` times."""
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            k, v, s = q8.pool(c["k"].copy(), "int8"), q8.pool(c["v"].copy(), "int8"), q8.on_gpu(c["s"].copy())
+            outs = []
+            for x in c["x"]:
+                q8.ft().kv_append_paged_q8(k, v, s, x, x, c["slots"])
+                outs.append(q8.ft().attention_decode_paged_q8(c["q"], k, v, s, c["table"], c["lens"]))
+        stream.synchronize()
+        return torch.stack(outs).cpu()
+    want = [work(c) for c in cases]
+    with ThreadPoolExecutor(3) as pool:
+        got = [f.result() for f in [pool.submit(work, c) for c in cases]]
+    assert all(w.shape == (calls, 3, 8, dim) and torch.equal(w, g) for w, g in zip(want, got)) and len(got) == 3

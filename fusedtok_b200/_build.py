@@ -50,47 +50,78 @@ def _out_of_date(target, source):
     return any(os.path.getmtime(d) > t for d in _includes(source))
 
 
-def stale(target=None):
-    target = target or LIB
-    return any(_out_of_date(target, os.path.join(CSRC, s)) for s in SOURCES)
+def _recipe(cmd):
+    """What decides on the result of `cmd` beside the sources: the command, wherever this tree lies, and its compiler's
+    version. None without the compiler: what is there then counts as made by it."""
+    try:
+        version = subprocess.run([cmd[0], "--version"], stdout=subprocess.PIPE, text=True, check=True).stdout
+    except FileNotFoundError:
+        return None
+    return "\n".join(a.replace(HERE, ".") for a in cmd) + "\n" + version
+
+
+def _stamp(target):
+    """File that holds the recipe `target` was made by."""
+    return os.path.join(OBJECTS, os.path.basename(target) + ".recipe")
+
+
+def _made_by(target, recipe):
+    if recipe is None or not os.path.exists(target) or not os.path.exists(_stamp(target)):
+        return recipe is None and os.path.exists(target)
+    with open(_stamp(target)) as f:
+        return f.read() == recipe
+
+
+def _run(jobs, began):
+    """Run `jobs` [(target, command, recipe)] side by side. What is built is dated from when the build began: an edit
+    made meanwhile leaves it out of date."""
+    jobs, running, failed = list(jobs), [], []
+    while jobs or running:
+        while jobs and len(running) < max(2, os.cpu_count() or 2):
+            target, cmd, recipe = jobs.pop(0)
+            if os.path.exists(_stamp(target)):
+                os.remove(_stamp(target))                 # (until the command has succeeded)
+            running.append((target, recipe, subprocess.Popen(cmd)))
+        target, recipe, job = running.pop(0)
+        try:
+            if job.wait(timeout=1) != 0:
+                failed.append(target)
+                continue
+            os.utime(target, (began, began))
+            with open(_stamp(target), "w") as f:
+                f.write(recipe)
+        except subprocess.TimeoutExpired:
+            running.append((target, recipe, job))
+    if failed:
+        raise RuntimeError("building failed for " + ", ".join(failed))
 
 
 def _compile(variants, force=False, verbose=False):
-    """Bring the objects of `variants` [(defines, target)] up to date, every source in an nvcc of its own side by
-    side, and link each variant's library. What is built is dated from when the build began: an edit made meanwhile
-    leaves it out of date."""
+    """Bring the libraries of `variants` [(defines, target)] up to date: objects whose source, included files, command or
+    compiler changed, every source in an nvcc of its own side by side, then the libraries whose objects or command did.
+    `verbose` compiles all objects, to report on each."""
     os.makedirs(OBJECTS, exist_ok=True)
     began = time.time()
-    jobs, linked = [], []
+    jobs, links = [], []
     for defines, target in variants:
         tag = "".join("_" + re.sub(r"\W", "_", d) for d in sorted(defines))
         objects = []
         for s in SOURCES:
             source, obj = os.path.join(CSRC, s), os.path.join(OBJECTS, s[:-3] + tag + ".o")
             objects.append(obj)
-            if force or _out_of_date(obj, source):
-                jobs.append((os.path.getsize(source), ["nvcc"] + NVCC_FLAGS + ["-D" + d for d in defines]
-                             + (["-Xptxas", "-v"] if verbose else []) + ["-c", source, "-o", obj]))
-        linked.append((objects, target))
+            cmd = ["nvcc"] + NVCC_FLAGS + ["-D" + d for d in defines] + ["-c", source, "-o", obj]
+            recipe = _recipe(cmd)
+            if force or verbose or not _made_by(obj, recipe) or _out_of_date(obj, source):
+                jobs.append((os.path.getsize(source), (obj, cmd + (["-Xptxas", "-v"] if verbose else []), recipe)))
+        links.append((objects, target))
     jobs.sort(key=lambda j: -j[0])                    # the longest first
-    running, failed = [], []
-    while jobs or running:
-        while jobs and len(running) < max(2, os.cpu_count() or 2):
-            cmd = jobs.pop(0)[1]
-            running.append((cmd, subprocess.Popen(cmd)))
-        cmd, job = running.pop(0)
-        try:
-            if job.wait(timeout=1) != 0:
-                failed.append(cmd[-1])
-            else:
-                os.utime(cmd[-1], (began, began))
-        except subprocess.TimeoutExpired:
-            running.append((cmd, job))
-    if failed:
-        raise RuntimeError("nvcc failed for " + ", ".join(failed))
-    for objects, target in linked:
-        subprocess.check_call(["nvcc"] + LINK_FLAGS + objects + ["-o", target])
-        os.utime(target, (began, began))
+    _run([j for _, j in jobs], began)
+    built = {j[0] for _, j in jobs}
+    for objects, target in links:
+        cmd = ["nvcc"] + LINK_FLAGS + objects + ["-o", target]
+        recipe = _recipe(cmd)
+        if built.intersection(objects) or not _made_by(target, recipe) or any(os.path.getmtime(o) > os.path.getmtime(target) for o in objects):
+            _run([(target, cmd, recipe)], began)
 
 
 # The module that makes plain calls straight from torch tensors (csrc/tensor_calls.cpp). An accelerator of the Python
@@ -101,15 +132,11 @@ BINDING = os.path.join(HERE, "_tensors.so")
 def build_binding(force=False):
     """Compile the module with the C++ headers of the installed torch; nothing to do without torch."""
     source = os.path.join(CSRC, "tensor_calls.cpp")
-    stamp = os.path.join(OBJECTS, "tensor_calls.torch")      # the torch it was built for
     try:
         import torch
         from torch.utils import cpp_extension
     except ImportError:
         return None
-    built_for = open(stamp).read() if os.path.exists(stamp) else ""
-    if not force and built_for == torch.__version__ and not _out_of_date(BINDING, source):
-        return BINDING
     began = time.time()
     root = os.path.dirname(torch.__file__)
     cuda = os.environ.get("CUDA_HOME") or cpp_extension.CUDA_HOME or "/usr/local/cuda"
@@ -118,21 +145,23 @@ def build_binding(force=False):
               os.path.join(cuda, "include"), sysconfig.get_paths()["include"]):
         cmd += ["-I", d]
     cmd += ["-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
-    if subprocess.call(cmd) != 0:
+    recipe = _recipe(cmd + [torch.__version__])
+    if not force and _made_by(BINDING, recipe) and not _out_of_date(BINDING, source):
+        return BINDING
+    os.makedirs(OBJECTS, exist_ok=True)
+    try:
+        _run([(BINDING, cmd, recipe)], began)
+    except RuntimeError:
         if os.path.exists(BINDING):
             os.remove(BINDING)
         print("fusedtok_b200: %s was not built; calls take the Python wrappers' way" % BINDING)
         return None
-    os.utime(BINDING, (began, began))
-    os.makedirs(OBJECTS, exist_ok=True)
-    with open(stamp, "w") as f:
-        f.write(torch.__version__)
     return BINDING
 
 
 def build_all(force=False):
     """The product and the self-checking variant, whichever is out of date, compiled side by side."""
-    _compile([(d, t) for d, t in (((), LIB), (("FTK_BOUNDS",), BOUNDS_LIB)) if force or stale(t)], force)
+    _compile([((), LIB), (("FTK_BOUNDS",), BOUNDS_LIB)], force)
     build_binding(force)
     return LIB
 
@@ -144,8 +173,6 @@ def build(force=False, verbose=False, defines=(), out=None):
     target = out or LIB
     if not defines:
         build_binding(force)
-    if not force and not defines and not stale():
-        return LIB
     _compile([(tuple(defines), target)], force, verbose)
     return target
 

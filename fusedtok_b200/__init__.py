@@ -675,9 +675,9 @@ def _host_slots(slots, n, blocks, page):
     if raw.size and raw.dtype.kind not in "iu":
         raise TypeError(f"slots: integer values expected, found {raw.dtype}")
     _index_shape("slots", raw.shape, (n,))
-    raw = raw.astype(np.int64)
     if raw.size and int(raw.max()) >= blocks * page:
         raise ValueError(f"slots: values must lie below {blocks * page} (found {int(raw.max())})")
+    raw = raw.astype(np.int64)                           # (now that a uint64 beyond it has been refused)
     raw = np.where(raw < 0, -1, raw)
     # first token of each run; no block may have two
     inside = (raw[1:] == raw[:-1] + 1) & (raw[1:] % page != 0) & (raw[:-1] >= 0)

@@ -657,8 +657,9 @@ def kv_append_paged_q8(k_pool, v_pool, kv_scales, k_new, v_new, slots):
     if blocks * page > 0x7fffffff:
         raise ValueError(f"k_pool: {blocks} blocks of {page} rows are more rows than a slot can name")
     if _on_gpu(slots):
-        if slots.dtype is torch.int64:               # (a slot that int32 cannot hold is outside the pool: keep it there)
-            slots = slots.clamp(-1, 0x7fffffff)
+        # A slot that int32 cannot hold is outside the pool: keep it there. (uint64 from 2^63 on is negative to int64.)
+        if slots.dtype in (torch.int64, torch.uint64):
+            slots = slots.view(torch.int64).clamp(-1, 0x7fffffff)
         where = call.index("slots", _whole("slots", slots), (n,), blocks * page, False)
     else:
         where = torch.from_numpy(_host_slots(slots, n, blocks, page)).to(call.device)

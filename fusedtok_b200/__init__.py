@@ -605,12 +605,14 @@ def attention_decode_paged_q8(q, k_pool, v_pool, kv_scales, block_table, lens=No
 
     ``out[b, h] = softmax_t(ks[t] * (q[b, h] . k8[t]) / sqrt(D)) . (vs[t] * v8[t])``, t over the sequence's rows
 
-    q ``[B, Hq, D]`` float32, bfloat16 or float16 (the result has its type, accumulation is float32); pools
-    ``[Nb, Hkv, P, D]`` of ``torch.int8`` or ``torch.float8_e4m3fn`` codes; kv_scales ``[Nb, Hkv, 2]`` float32: K's
-    scale, then V's (``kv_append_paged_q8`` fills both); block_table ``[B, S]`` and lens ``[B]`` as in
-    ``attention_decode_paged``. Any GQA group. The V scales of one sequence's blocks may differ by a factor of up to
-    2^60. CUDA tensors only; host table and lens values are checked, CUDA tensors trusted. The scratch of a call comes
-    from torch's allocator, so calls on different streams do not share any. No counterpart in the reference."""
+    q ``[B, Hq, D]`` float32, bfloat16 or float16 (the result has its type; softmax statistics and sums are float32,
+    and what goes to the tensor cores in half precision, softmax weights and float32 queries, goes in two parts that
+    keep 22 bits); pools ``[Nb, Hkv, P, D]`` of ``torch.int8`` or ``torch.float8_e4m3fn`` codes; kv_scales
+    ``[Nb, Hkv, 2]`` float32: K's scale, then V's (``kv_append_paged_q8`` fills both); block_table ``[B, S]`` and lens
+    ``[B]`` as in ``attention_decode_paged``. Any GQA group. The V scales of one sequence's blocks, those that are zero
+    aside, may differ by a factor of up to 2^60. CUDA tensors only; host table and lens values are checked, CUDA
+    tensors trusted. The scratch of a call comes from torch's allocator, so calls on different streams do not share
+    any. No counterpart in the reference."""
     out = _decode_q8_native(q, k_pool, v_pool, kv_scales, block_table, lens)
     if out is not None:
         return out
@@ -748,7 +750,8 @@ def block_table_extend(block_table, lens, new_lens, free_blocks, free_count, pag
 def block_table_trim(block_table, lens, keep_lens, free_blocks, free_count, page):
     """Cut sequences back to ``min(lens[b], keep_lens[b])`` tokens (0: finished, or a shorter length: rejected draft
     tokens) and push the blocks that they no longer need on the free stack, in batch order, from
-    ``free_blocks[free_count]`` on. Returns ``(lens, free_count)``, the new lengths and count; the table is only read.
+    ``free_blocks[free_count]`` on (as many as it has room for). Returns ``(lens, free_count)``, the new lengths and
+    count; the table is only read.
     Operands as in :func:`block_table_extend`. No counterpart in the reference."""
     cut = _trim_native(block_table, lens, keep_lens, free_blocks, free_count, page)
     if cut is not None:

@@ -16,12 +16,14 @@
 //  * 2 helper warps prepare the query fragments of the next segments, 2 fold the 8 states of the last ones. With both done
 //    by the consumers, and barriers between them, every segment cost a CTA about 4 us (12 tiles' worth), and 64 ragged
 //    sequences took 130 us instead of 90.
-// Measured (B200, back to back in a graph, 3 % more under sustained power): 32 sequences x 4096 rows, 32 / 8 heads of 128,
-// bf16 and int8: 49.5 us, 5.4 TB/s; 64 ragged ones of 128 - 8192 rows, fp16 and e4m3: 89 us, 6.1 TB/s; 4 x 131072 rows, 64 / 8
-// heads, bf16 and e4m3: 164 us, 6.5 TB/s, the copy rate. What is left of the first is its ends: 3.3 us from the release of
-// the launch to the first copy (lengths read, ranges located, table entries read), 1.5 us from a CTA's last tile to its
-// exit, 2.7 us for the merge behind. Consumers are the limit from 16 heads per kv head (68 us) and, with 16-row blocks of
-// 64-wide heads, the rate of 1 KB copies (60 us; 52 us with 64-row blocks).
+// Measured (B200, back to back in a graph; called one behind the other for long 4 to 6 % more, the third 4 to 13 %, by what
+// the power cap leaves of the clock): 32 sequences x 4096 rows, 32 / 8 heads of 128, bf16 and int8: 49.7 us, 5.4 TB/s; 64 ragged ones of
+// 128 - 8192 rows, fp16 and e4m3: 90 us, 6.1 TB/s; 4 x 131072 rows, 64 / 8 heads, bf16 and e4m3: 165 us, 6.5 TB/s, the copy
+// rate. What is left of the first is its ends: 3.3 us from the release of the launch to the first copy (lengths read, ranges
+// located, table entries read), 1.5 us from a CTA's last tile to its exit, 2.7 us for the merge behind. With 16 heads per kv
+// head (83 us) the consumers are the limit: the issue slots are 42 % busy, the tensor pipe 29 %, and two consumer warps a
+// scheduler are too few to cover what each waits for. With 16-row blocks of 64-wide heads it is the rate of 1 KB copies (61 us;
+// 53 us with 64-row blocks).
 //  * Stage layout: a block's (page x D) bytes are contiguous in the pool, so the pool is described to TMA as 128-byte
 //    lines with the 128-byte swizzle, whatever D is; row r, 16-byte chunk c of a tile sits at line-linear address
 //    r * D + 16 c, swizzled. One copy per block and tile for K, one for V; the two scales of the block follow with an
@@ -44,8 +46,8 @@
 //    SPLIT: with at most 4 query heads per unit (8 with two column blocks) each head takes two of the 8 MMA columns for the two
 //    parts of q and of the weights, at no cost in MMAs. float32 calls always run this way (q needs 22 bits too), 16-bit calls
 //    when their heads fit. Without SPLIT q, 16 bits as it is, goes in one half, and the remainders of the weights take an MMA
-//    of their own into the same accumulators: with 8 heads per kv head 53.7 us instead of 52.8 (32 x 4096 rows), with 16 79.4
-//    instead of 72.8.
+//    of their own into the same accumulators: with 8 heads per kv head 53.7 us instead of 52.8 (32 x 4096 rows, captured; 4 x
+//    131072 rows called for long, under the power cap, 172 - 187 us instead of 167 - 177), with 16 79.4 instead of 72.8.
 //  * A unit that lies in one range is finished in place. Otherwise the CTAs leave (m, l, acc) partials, at most two per
 //    range, in a workspace that belongs to the call, and q8_merge_kernel, launched behind with programmatic stream
 //    serialization, folds them in range order. No counters, no state between calls: calls on different streams, and

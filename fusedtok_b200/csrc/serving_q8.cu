@@ -102,8 +102,10 @@ Q8Plan plan_q8(int dtype, int batch, int hq, int hkv, int page, int width, int d
         pl.GC = std::min(G, pl.nbk * per);
         pl.NCH = (G + pl.GC - 1) / pl.GC;
         pl.units = (long long)batch * hkv * pl.NCH;
-        // Units of up to 8 tiles stay whole while there are no more of them than SMs: a CTA works through 8 tiles in less
-        // time than partials and their merge take (8 heads x 512 rows: 7.2 us on 8 CTAs, 9.0 on 64; with 16 tiles 11.7 and 10.4)
+        // As many CTAs as units where those have at most 8 tiles and are no more than the SMs: with equal lengths every unit is
+        // then one CTA's, which works through 8 tiles in less time than partials and their fold take (8 heads of 64 x 512 rows:
+        // 7.2 us on 8 CTAs, 9.2 on 64). Unequal lengths are cut at equal cost all the same, into fewer parts. With 16 tiles heads
+        // of 64 would still gain (9.0 and 9.8); larger heads and groups, whose tiles take longer, were not measured there.
         pl.ncta = (int)(tiles <= 8 && pl.units <= sms ? pl.units : std::max<long long>(1, std::min<long long>(sms, pl.units * tiles)));
         for (pl.box_shift = 4; (1 << pl.box_shift) < std::min(page, TILE);) ++pl.box_shift;
         const size_t slots = (size_t)2 * pl.ncta;
@@ -251,8 +253,8 @@ int fusedtok_attention_decode_paged_q8_launch(int dtype, int store, const void* 
     if ((rc = status_word(&p.device, &p.status))) return rc;
     cudaError_t e = cudaSuccess;
     // Blocks per unit of the merge: one for every 128 sums where that makes no more of them than SMs (4 sequences of 571 - 2061
-    // rows, 4 kv heads: with 16 heads each 19.3 us instead of 21.7, with 8 13.5 instead of 14.4), else one (32 x 4096 rows, 8 kv heads
-    // of 16: 71.9 us, and 75.0 with four: blocks without a unit to merge hold the next launch up)
+    // rows, 4 kv heads: with 16 heads each 20.3 us instead of 22.8, with 8 14.1 instead of 14.8), else one (32 x 4096 rows, 8 kv heads
+    // of 16: 82.2 us, and 85.3 with four: blocks without a unit to merge hold the next launch up)
     const long long per_unit = (pl.GC * (dim / 4) + Q8M_TEAM - 1) / Q8M_TEAM;
     const unsigned slices = pl.units * per_unit <= sms ? (unsigned)per_unit : 1u;
     if (pl.tc) {

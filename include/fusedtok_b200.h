@@ -299,8 +299,11 @@ int fusedtok_attention_decode_launch_noalloc(int dtype, const void* q, const voi
  *
  * attention_decode_paged_q8: fusedtok_attention_decode_paged_launch over such a
  * cache (same shapes, head mapping, scale and zero rows; any GQA group; a block
- * table entry outside [0, num_blocks) is read as block 0). Accumulation in float32;
- * the V scales of one sequence's blocks may differ by a factor of up to 2^60.
+ * table entry outside [0, num_blocks) is read as block 0). Softmax statistics and
+ * sums in float32; what goes to the tensor cores in half precision, softmax weights
+ * and float32 queries, goes in two parts that keep 22 bits, and a weight is lost
+ * below 2^-39 of the largest weight * V scale. The V scales of one sequence's
+ * blocks, those that are zero aside, may differ by a factor of up to 2^60.
  * `workspace`: 16-byte aligned device memory of at least
  * fusedtok_attention_decode_paged_q8_workspace(...) bytes that the call may
  * overwrite and no other work may touch until it is done (its contents before
@@ -352,7 +355,7 @@ int fusedtok_kv_append_paged_q8_launch(int dtype, int store, const void* k_new, 
  *
  * trim: b is cut back to min(lens[b], keep_lens[b]) tokens (0: finished). The
  * blocks no longer needed are pushed in batch order: free_blocks[*free_count],
- * ...; lens_out and *free_count_out are the new lengths and count. The table is
+ * ..., as many as free_capacity has room for; lens_out and *free_count_out are the new lengths and count. The table is
  * only read; its entries behind the new lengths stand for nothing.
  *
  * Negative lengths count as 0. At most 8192 sequences. lens_out and

@@ -40,7 +40,8 @@
 //    factor half precision ends at 2^-25, and thousands of rows 17 natural log units below one row, whose sum is
 //    what there is to see when that row's V is small, were lost altogether.) e is counted from a warp's first block that is not zero, so that
 //    both stay in range as long as the V scales of a sequence differ by less than 2^60 (those that are zero aside, which set no
-//    exponent and leave w to the others).
+//    exponent). A block more than 2^60 above that one moves e's zero up; blocks more than 2^60 below the largest keep their
+//    part in l, and in O what is left of it.
 //  * A weight goes to the tensor cores in two halves, its value rounded to half and the remainder: 22 bits, whatever the type of
 //    q. Rounded once (2^-12 of the weight at most) it added as much error to a float16 result as the result's own rounding.
 //    SPLIT: with at most 4 query heads per unit (8 with two column blocks) each head takes two of the 8 MMA columns for the two
@@ -507,8 +508,9 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     float acc[NBK][KSTEPS][4];                     // O^T block mt: d = 16 mt + 2 quad ([0], [1]) and + 1 ([2], [3])
     float kf[NBK][HPT];                            // score factor of the head: its row's exponent / sqrt(D) * log2(e)
     float m_run[NBK][HPT], l_run[NBK][HPT];        // R of the head; this thread's share of l
-    // biased exponent that this warp counts V scales from; negative: only blocks of zeros so far, 0: no rows
-    int e0 = 0, top = 0;                           // top: largest exponent so far, counted from e0
+    // biased exponent that this warp counts V scales from (-127: only blocks of zeros so far, -126: no rows), and the largest
+    // exponent so far, counted from there
+    int e0 = -126, top = 0;
 
     // Byte offset of chunk 2 i + csel of row r inside a tile, swizzled. `csel` and the row are the lane's.
     const int lrow = ((lane >> 3) & 1) * 8 + (lane & 7), csel = lane >> 4;
@@ -565,28 +567,54 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 #pragma unroll
         for (int n = 0; n < PF; ++n) ldsm_x4_t(st_v + chunk_off(n / NLD, n % NLD), f[n][0], f[n][1], f[n][2], f[n][3]);
         // ---- online softmax, in units of log2
-        if (e0 <= 0) {
-            e0 = -127;                   // (a block of zeros says nothing about the others)
-            top = 0;
+        // Exponents of the blocks' vs less e0: at most 60. Otherwise (and always while e0 is negative) there is something to settle
+        int d[RB], hi = -255;
 #pragma unroll
-            for (int j = RB - 1; j >= 0; --j)
-                if (ks[j].y != 0.0f) e0 = min(max((int)(__float_as_uint(ks[j].y) >> 23 & 255u), 61), 194);
+        for (int j = 0; j < RB; ++j) {
+            d[j] = (int)(__float_as_uint(ks[j].y) >> 23 & 255u) - e0;
+            hi = max(hi, d[j]);
         }
-        // Per block: exponent of vs less e0 (e0 + d covers 1 .. 254, every finite scale), 2^-that, and what is left of vs. Rows of a
-        // block of zeros add to l alone and only have to keep R in range of their s: they count as 60 below the others
+        if (hi > 60) {
+            if (e0 < 0) {                // a block of zeros says nothing about the others: the first that is not one sets e0
+                top = 0;
+                e0 = -127;
+#pragma unroll
+                for (int j = RB - 1; j >= 0; --j)
+                    if (ks[j].y != 0.0f) e0 = min(max((int)(__float_as_uint(ks[j].y) >> 23 & 255u), 61), 194);
+            }
+            hi = -255;
+#pragma unroll
+            for (int j = 0; j < RB; ++j) {
+                d[j] = min((int)(__float_as_uint(ks[j].y) >> 23 & 255u), 254) - abs(e0);
+                hi = max(hi, d[j]);
+            }
+            if (hi > 60) {               // e0 moves up, and R with it
+                const int by = hi - 60;
+                const float f = __uint_as_float((uint32_t)(127 + by / 2) << 23), g = __uint_as_float((uint32_t)(127 + by - by / 2) << 23);
+                e0 += by;
+                top -= by;
+                hi = 60;
+#pragma unroll
+                for (int j = 0; j < RB; ++j) d[j] -= by;
+#pragma unroll
+                for (int nbk = 0; nbk < NBK; ++nbk)
+#pragma unroll
+                    for (int e = 0; e < HPT; ++e) {
+                        m_run[nbk][e] -= (float)by;
+                        l_run[nbk][e] = l_run[nbk][e] * f * g;
+                    }
+            }
+        }
+        // Per block: that exponent, 2^-it, and what is left of vs (e0 + d covers 1 .. 254, every finite scale). Rows 60 and more below
+        // the largest, those of a block of zeros among them, add to l and only have to keep R in range of their s
+        top = max(top, hi);
         float de[RB], ge[RB], ce[RB];
-        int d[RB];
 #pragma unroll
         for (int j = 0; j < RB; ++j) {
-            d[j] = min(max((int)(__float_as_uint(ks[j].y) >> 23 & 255u) - abs(e0), -60), 60);
-            top = max(top, d[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < RB; ++j) {
-            if (ks[j].y == 0.0f) d[j] = top - 60;
+            d[j] = max(d[j], top - 60);
             de[j] = (float)d[j];
             ge[j] = __uint_as_float((uint32_t)(127 - d[j]) << 23);
-            ce[j] = ks[j].y * __uint_as_float(max((uint32_t)(254 - (abs(e0) + d[j])) << 23, 0x00400000u)) * Q8_ROOM;
+            ce[j] = ks[j].y * __uint_as_float(max((uint32_t)(254 - abs(e0) - d[j]) << 23, 0x00400000u)) * Q8_ROOM;
         }
         uint32_t pb[NBK][RB][2];
         [[maybe_unused]] uint32_t pr[SPLIT ? 1 : NBK][RB][2];      // what the rounding to half left of the weights
@@ -692,7 +720,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         const int n = (int)(left < (long long)(w.nt - w.ti) ? left : (long long)(w.nt - w.ti));
         const bool mine = own < i0 + n;            // this group has a tile of the segment
         // ---- the segment's query fragments
-        e0 = 0;
+        e0 = -126;
         {
             const int buf = k % Cfg::NQ;
             mbar_wait(bar_q_full + buf * 8, (uint32_t)((k / Cfg::NQ) & 1), abort_flag, p.status, ST_WAIT_RANGE_TIMEOUT);
@@ -760,7 +788,7 @@ decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
                     const int le = (int)(__float_as_uint(l) >> 23) - 127, k = le > 32 ? le - 32 : le < -32 ? le + 32 : 0;
                     const float back = __uint_as_float((uint32_t)(127 - k) << 23);
                     if (quad == 0) s_ml[warp * HEADS + g] = make_float2(m_run[nbk][e] + (float)k, l * back);
-                    if (e0 != 0) {
+                    if (e0 != -126) {
                         float* my = s_acc + ((size_t)warp * HEADS + g) * Cfg::ACC_STRIDE + quad * 2;
 #pragma unroll
                         for (int mt = 0; mt < KSTEPS; ++mt) {

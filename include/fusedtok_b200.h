@@ -302,7 +302,8 @@ int fusedtok_attention_decode_launch_noalloc(int dtype, const void* q, const voi
  * table entry outside [0, num_blocks) is read as block 0). Softmax statistics and
  * sums in float32; what goes to the tensor cores in half precision, softmax weights
  * and float32 queries, goes in two parts that keep 22 bits, and a weight is lost
- * below 2^-39 of the largest weight * V scale. The V scales of one sequence's
+ * below 2^-39 of the largest weight * V scale (a scale of zero counting as 2^-60 of
+ * the largest). The V scales of one sequence's
  * blocks, those that are zero aside, may differ by a factor of up to 2^60.
  * `workspace`: 16-byte aligned device memory of at least
  * fusedtok_attention_decode_paged_q8_workspace(...) bytes that the call may

@@ -181,3 +181,20 @@ def test_v_scales_and_scores_far_apart(case, hq, dim, store):
     # the same blocks many times over: units that are cut, and folded by the merge
     table = np.repeat(table, 40, axis=0).reshape(1, -1)
     check(torch.ones((1, hq, dim)), k, v, scales, table, [16 * table.shape[1]], store, "f32")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("store", list(q8.STORES))
+@pytest.mark.parametrize("hq,dim", [(4, 128), (8, 64), (3, 256), (16, 96)])
+@pytest.mark.parametrize("spread", [61, 66, 75, 90, 120, 150])
+def test_v_scales_beyond_the_range_that_is_promised(spread, hq, dim, store):
+    """V scales further apart than 2^60, smallest and largest first, with scores that do not make up for it: the large ones
+    decide, and the weights of the others count below the line."""
+    rng = np.random.default_rng(spread)
+    for order in (1, -1):
+        powers = np.concatenate([np.linspace(-spread / 2, spread / 2, 12).round(), [-spread // 2, 0, spread // 2, None]])[::order]
+        scores = rng.uniform(-4, 4, len(powers)).round(2)
+        k, v, scales, table = rows_of_one_score(scores, [None if e is None else int(e) for e in powers], dim, store, rng)
+        for n in (1, 40):
+            wide = np.repeat(table, n, axis=0).reshape(1, -1)
+            check(torch.ones((1, hq, dim)), k, v, scales, wide, [16 * wide.shape[1]], store, "f32")

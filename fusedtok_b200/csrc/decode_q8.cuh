@@ -23,7 +23,7 @@
 // located, table entries read), 1.5 us from a CTA's last tile to its exit, 2.7 us for the merge behind. With 16 heads per kv
 // head (83 us) the consumers are the limit: the issue slots are 42 % busy, the tensor pipe 29 %, and two consumer warps a
 // scheduler are too few to cover what each waits for. With 16-row blocks of 64-wide heads it is the rate of 1 KB copies (61 us;
-// 53 us with 64-row blocks).
+// 54 us with 64-row blocks).
 //  * Stage layout: a block's (page x D) bytes are contiguous in the pool, so the pool is described to TMA as 128-byte
 //    lines with the 128-byte swizzle, whatever D is; row r, 16-byte chunk c of a tile sits at line-linear address
 //    r * D + 16 c, swizzled. One copy per block and tile for K, one for V; the two scales of the block follow with an
